@@ -18,11 +18,13 @@ TSDF_PATH = LIB_DIR / ("libnavi_tsdf_debug.so" if os.environ.get("NAVI_TSDF_DEBU
                        else "libnavi_tsdf.so")
 GMDAG_PATH = LIB_DIR / "libnavi_gmdag.so"
 GMDAG_GPU_PATH = LIB_DIR / "libnavi_gmdag_gpu.so"
+POLICY_PATH = LIB_DIR / "libnavi_policy.so"
 
 _lock = threading.Lock()
 _tsdf: ctypes.CDLL | None = None
 _gmdag: ctypes.CDLL | None = None
 _gmdag_gpu: ctypes.CDLL | None = None
+_policy: ctypes.CDLL | None = None
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -162,6 +164,72 @@ GMDAG_GPU_SIGNATURES: dict[str, tuple[object, list[object]]] = {
 }
 
 
+c_int32 = ctypes.c_int32
+Strides = c_int64 * 3
+
+
+class PolicyAttention(ctypes.Structure):
+    """policy_attention of include/policy.h."""
+
+    _fields_ = [
+        ("device", c_int32), ("dtype", c_int32),
+        ("batch", c_int64), ("lq", c_int64), ("lk", c_int64),
+        ("heads", c_int32), ("kv_heads", c_int32), ("dim", c_int32),
+        ("scale", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_strides", Strides), ("k_strides", Strides), ("v_strides", Strides),
+        ("key_mask", c_void_p), ("key_mask_stride", c_int64), ("key_lengths", c_void_p),
+        ("out", c_void_p), ("lse", c_void_p),
+        ("dout", c_void_p), ("dout_strides", Strides),
+        ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+        ("workspace", c_void_p),
+    ]
+
+
+class PolicyNormSide(ctypes.Structure):
+    """policy_norm_side of include/policy.h."""
+
+    _fields_ = [
+        ("x", c_void_p), ("strides", Strides), ("tokens", c_int64),
+        ("heads", c_int32), ("reserved", c_int32),
+        ("weight", c_void_p), ("table", c_void_p), ("table_rows", c_int64), ("positions", c_void_p),
+        ("y", c_void_p), ("dy", c_void_p), ("dy_strides", Strides), ("dx", c_void_p), ("dweight", c_void_p),
+    ]
+
+
+class PolicyQkNorm(ctypes.Structure):
+    """policy_qk_norm of include/policy.h."""
+
+    _fields_ = [
+        ("device", c_int32), ("dtype", c_int32), ("batch", c_int64), ("dim", c_int32), ("rotary", c_int32),
+        ("eps", c_float), ("reserved", c_int32), ("side", PolicyNormSide * 2), ("workspace", c_void_p),
+    ]
+
+
+class PolicyGrad(ctypes.Structure):
+    """policy_grad of include/policy.h."""
+
+    _fields_ = [("grad", c_void_p), ("out", c_void_p), ("count", c_uint64), ("dtype", c_int32), ("reserved", c_int32)]
+
+
+POLICY_F32 = 0  # policy_dtype of include/policy.h
+POLICY_BF16 = 1
+
+# name -> (restype, argtypes); mirrors include/policy.h
+POLICY_SIGNATURES: dict[str, tuple[object, list[object]]] = {
+    "policy_version": (c_int, []),
+    "policy_last_error": (c_char_p, []),
+    "policy_cross_attention_workspace_bytes": (c_uint64, [ctypes.POINTER(PolicyAttention), c_int]),
+    "policy_cross_attention": (c_int, [ctypes.POINTER(PolicyAttention), c_void_p]),
+    "policy_cross_attention_backward": (c_int, [ctypes.POINTER(PolicyAttention), c_void_p]),
+    "policy_qk_norm_workspace_bytes": (c_uint64, [ctypes.POINTER(PolicyQkNorm)]),
+    "policy_qk_norm_rotary": (c_int, [ctypes.POINTER(PolicyQkNorm), c_void_p]),
+    "policy_qk_norm_rotary_backward": (c_int, [ctypes.POINTER(PolicyQkNorm), c_void_p]),
+    "policy_clip_grad_workspace_bytes": (c_uint64, [ctypes.POINTER(PolicyGrad), c_int64]),
+    "policy_clip_grad_norm": (c_int, [ctypes.POINTER(PolicyGrad), c_int64, c_float, c_void_p, c_int, c_void_p, c_void_p]),
+}
+
+
 def _bind(lib: ctypes.CDLL, sigs: dict[str, tuple[object, list[object]]]) -> None:
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -215,6 +283,28 @@ def gmdag_gpu_lib() -> ctypes.CDLL:
                 _bind(lib, GMDAG_GPU_SIGNATURES)
                 _gmdag_gpu = lib
     return _gmdag_gpu
+
+
+def policy_lib() -> ctypes.CDLL:
+    """The policy operators; raises RuntimeError when the library is not built or cannot load."""
+    global _policy
+    if _policy is None:
+        with _lock:
+            if _policy is None:
+                if not POLICY_PATH.exists():
+                    raise RuntimeError(
+                        f"navi_b200 policy operators not found at {POLICY_PATH}; run `python -m navi_b200.build`"
+                    )
+                lib = ctypes.CDLL(str(POLICY_PATH))
+                _bind(lib, POLICY_SIGNATURES)
+                _policy = lib
+    return _policy
+
+
+def check_policy(rc: int, what: str) -> None:
+    if rc != 0:
+        msg = policy_lib().policy_last_error()
+        raise RuntimeError(f"{what} failed ({rc}): {msg.decode() if msg else ''}")
 
 
 def last_error() -> str:

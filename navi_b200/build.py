@@ -10,9 +10,10 @@
                      that its float arithmetic matches the reference compiler's)
 - libnavi_gmdag_gpu.so : the device scene compiler (nvcc sm_100a, -fmad=false,
                      IEEE division / sqrt; same words as libnavi_gmdag.so)
+- libnavi_policy.so : the policy operators and the C ABI of include/policy.h (nvcc sm_100a)
 - libnavi_probe.so : the L2 read-bandwidth probe of the benchmark's roofline
 
-Both are rebuilt only when a source is newer than the library.
+All are rebuilt only when a source is newer than the library.
 """
 
 from __future__ import annotations
@@ -120,6 +121,23 @@ def build_gmdag_gpu(force: bool = False) -> Path:
     return out
 
 
+def build_policy(force: bool = False) -> Path:
+    """libnavi_policy.so: cross attention, norms of queries and keys with rotation, gradient clipping."""
+    out = LIB / "libnavi_policy.so"
+    srcs = [CSRC / "policy_attention.cu", CSRC / "policy_norm.cu", CSRC / "policy_clip.cu", CSRC / "policy_common.cpp"]
+    deps = srcs + [CSRC / "policy_internal.h", CSRC / "policy_mma.cuh", INCLUDE / "policy.h"]
+    if force or _stale(out, deps):
+        LIB.mkdir(parents=True, exist_ok=True)
+        tmp = out.with_suffix(".so.tmp")
+        _run([
+            _nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
+            "-Xcompiler", "-fvisibility=hidden", "-Xlinker", "--exclude-libs,ALL", "--threads", "0",
+            f"-I{INCLUDE}", *map(str, srcs), "-o", str(tmp),
+        ])
+        tmp.replace(out)
+    return out
+
+
 def build_probe(force: bool = False) -> Path:
     """libnavi_probe.so: the L2 read-bandwidth probe bench.py reports the L2 roofline against,
     and the check of the trace kernel's exit quotient against the IEEE division."""
@@ -136,7 +154,7 @@ def build_probe(force: bool = False) -> Path:
 
 def build_all(force: bool = False) -> list[Path]:
     return [build_tsdf(force), build_tsdf(force, bounds_check=True), build_gmdag(force), build_gmdag_gpu(force),
-            build_probe(force)]
+            build_policy(force), build_probe(force)]
 
 
 if __name__ == "__main__":

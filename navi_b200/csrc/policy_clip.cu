@@ -1,0 +1,282 @@
+// The global norm of a list of gradients, and their clipping.
+//
+// Two launches: every block adds the squares of its chunks (32 bits within a thread's chunk, 64 bits
+// from there on) into one partial sum; every block of the second launch adds the partial sums in the
+// same order, which costs it a few kilobytes from L2 and saves a launch between the two, and scales
+// its chunks.  Memory bounds both; the second pass takes the chunks in the opposite order, so that it
+// starts on what the first left in L2.
+#include <cuda_bf16.h>
+
+#include <limits>
+#include <new>
+
+#include "policy_internal.h"
+
+namespace policy {
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr int kThreads = 256;
+constexpr int kChunk = 4096;        // values: 16 per thread
+constexpr int kBlocksPerSm = 8;     // 256 threads: the SM is full
+constexpr int kMaxSms = 256;         // SMs that the workspace allows for
+constexpr int kTensors = 512;       // tensors of one launch (its parameters)
+
+struct ClipTensor {
+    const void* grad;
+    void* out;
+    uint64_t count;
+    uint32_t first_chunk;  // chunks of the launch's tensors before this one
+    uint32_t dtype;        // bit 0: bf16; bit 1: every chunk is 16-byte aligned
+};
+
+struct ClipParams {
+    ClipTensor t[kTensors];
+    double* parts;
+    float* norm;
+    float max_norm;
+    int n;
+    uint32_t chunks;
+    int part0;   // first partial sum of this launch (first pass)
+    int n_parts; // all partial sums (second pass)
+};
+
+__device__ __forceinline__ int find_tensor(const ClipParams& p, uint32_t chunk)
+{
+    int lo = 0, hi = p.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.t[mid].first_chunk <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double block_sum(double x)
+{
+    __shared__ double warp_sums[kThreads / 32];
+    __shared__ double total;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        x = 0.0;
+        for (int i = 0; i < kThreads / 32; ++i) x += warp_sums[i];
+        total = x;
+    }
+    __syncthreads();
+    return total;
+}
+
+__device__ __forceinline__ float2 unpack(uint32_t w)
+{
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+__device__ __forceinline__ uint32_t scale2(uint32_t w, float c)
+{
+    const float2 v = unpack(w);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x * c, v.y * c);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_constant__ ClipParams p)
+{
+    double sum = 0.0;
+    for (uint32_t chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
+        const ClipTensor& t = p.t[find_tensor(p, chunk)];
+        const uint64_t at = static_cast<uint64_t>(chunk - t.first_chunk) * kChunk;
+        const int n = static_cast<int>(min(static_cast<uint64_t>(kChunk), t.count - at));
+        float x = 0.f;
+        if (n == kChunk && (t.dtype & 2u)) {
+            if (t.dtype & 1u) {
+                const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.grad) + at);
+                uint4 v[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) v[i] = g[threadIdx.x + i * kThreads];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = unpack(w[k]);
+                        x = fmaf(f.x, f.x, fmaf(f.y, f.y, x));
+                    }
+                }
+            } else {
+                const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
+                float4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, fmaf(v[i].z, v[i].z, fmaf(v[i].w, v[i].w, x))));
+            }
+        } else {
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                const float v = (t.dtype & 1u) ? __bfloat162float(static_cast<const bf16*>(t.grad)[at + i])
+                                               : static_cast<const float*>(t.grad)[at + i];
+                x = fmaf(v, v, x);
+            }
+        }
+        sum += x;
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) p.parts[p.part0 + blockIdx.x] = sum;
+}
+
+__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ ClipParams p)
+{
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < p.n_parts; i += kThreads) sum += p.parts[i];
+    const float norm = static_cast<float>(sqrt(block_sum(sum)));
+    if (p.norm && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = norm;
+    const float f = p.max_norm / (norm + 1e-6f);
+    const float c = f > 1.f ? 1.f : f;  // NaN stays NaN
+    for (uint32_t k = blockIdx.x; k < p.chunks; k += gridDim.x) {
+        const uint32_t chunk = p.chunks - 1 - k;
+        const ClipTensor& t = p.t[find_tensor(p, chunk)];
+        if (c == 1.f && t.out == t.grad) continue;
+        const uint64_t at = static_cast<uint64_t>(chunk - t.first_chunk) * kChunk;
+        const int n = static_cast<int>(min(static_cast<uint64_t>(kChunk), t.count - at));
+        if (n == kChunk && (t.dtype & 2u)) {
+            if (t.dtype & 1u) {
+                const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.grad) + at);
+                uint4* o = reinterpret_cast<uint4*>(static_cast<bf16*>(t.out) + at);
+                uint4 v[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) v[i] = g[threadIdx.x + i * kThreads];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    o[threadIdx.x + i * kThreads] = make_uint4(scale2(v[i].x, c), scale2(v[i].y, c), scale2(v[i].z, c), scale2(v[i].w, c));
+            } else {
+                const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
+                float4* o = reinterpret_cast<float4*>(static_cast<float*>(t.out) + at);
+                float4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[threadIdx.x + i * kThreads] = make_float4(v[i].x * c, v[i].y * c, v[i].z * c, v[i].w * c);
+            }
+        } else {
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                if (t.dtype & 1u)
+                    static_cast<bf16*>(t.out)[at + i] = __float2bfloat16_rn(__bfloat162float(static_cast<const bf16*>(t.grad)[at + i]) * c);
+                else
+                    static_cast<float*>(t.out)[at + i] = static_cast<const float*>(t.grad)[at + i] * c;
+            }
+        }
+    }
+}
+
+// --- host ----------------------------------------------------------------------
+
+int check_grads(const policy_grad* grads, int64_t n)
+{
+    if (n < 0 || n > (1 << 24)) return fail(POLICY_ERR_INVALID, "n must be between 0 and 2^24");
+    if (n > 0 && !grads) return fail(POLICY_ERR_INVALID, "grads must not be null");
+    for (int64_t i = 0; i < n; ++i) {
+        const policy_grad& g = grads[i];
+        if (!known_dtype(g.dtype)) return fail(POLICY_ERR_INVALID, "dtype must be POLICY_F32 or POLICY_BF16");
+        if (g.count > (1ull << 40)) return fail(POLICY_ERR_INVALID, "count must not pass 2^40");
+        if (g.count && (!g.grad || !g.out)) return fail(POLICY_ERR_INVALID, "grad and out must not be null");
+        const size_t e = dtype_bytes(g.dtype);
+        if (reinterpret_cast<uintptr_t>(g.grad) % e || reinterpret_cast<uintptr_t>(g.out) % e)
+            return fail(POLICY_ERR_INVALID, "grad and out must be aligned to their type");
+    }
+    return POLICY_OK;
+}
+
+// Takes tensors from grads[i..] for one launch; returns how many entries it consumed.
+int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams& p)
+{
+    p.n = 0;
+    uint64_t chunks = 0;
+    int64_t i = 0;
+    for (; i < n && p.n < kTensors; ++i) {
+        const policy_grad& g = grads[i];
+        if (g.count == 0) continue;
+        const uint64_t own = (g.count + kChunk - 1) / kChunk;
+        if (chunks + own > std::numeric_limits<int32_t>::max()) break;  // one tensor alone always fits: count <= 2^40
+        ClipTensor& t = p.t[p.n++];
+        const bool wide = reinterpret_cast<uintptr_t>(g.grad) % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
+        t.grad = g.grad, t.out = g.out, t.count = g.count;
+        t.first_chunk = static_cast<uint32_t>(chunks);
+        t.dtype = (g.dtype == POLICY_BF16 ? 1u : 0u) | (wide ? 2u : 0u);
+        chunks += own;
+    }
+    p.chunks = static_cast<uint32_t>(chunks);
+    return i;
+}
+
+int launch_blocks(const ClipParams& p, int sms)
+{
+    const uint32_t most = static_cast<uint32_t>(sms < kMaxSms ? sms : kMaxSms) * kBlocksPerSm;
+    return static_cast<int>(p.chunks < most ? p.chunks : most);
+}
+
+int run_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, int device, void* workspace, cudaStream_t stream)
+{
+    int rc = check_grads(grads, n);
+    if (rc != POLICY_OK) return rc;
+    if (!(max_norm >= 0.f)) return fail(POLICY_ERR_INVALID, "max_norm must not be negative");
+    if (!norm) return fail(POLICY_ERR_INVALID, "norm must not be null");
+    const DeviceInfo info = device_info(device);
+    if (info.status != POLICY_OK) return info.status;
+    DeviceScope scope(device);
+    if (scope.error() != cudaSuccess) return cuda_fail(scope.error(), "cudaSetDevice");
+    ClipParams p;
+    p.parts = static_cast<double*>(workspace);
+    p.max_norm = max_norm;
+    p.n_parts = 0;
+    for (int64_t i = 0; i < n;) {
+        i += fill_launch(grads + i, n - i, p);
+        if (p.chunks == 0) continue;
+        if (!workspace) return fail(POLICY_ERR_INVALID, "workspace must not be null");
+        p.part0 = p.n_parts;
+        const int blocks = launch_blocks(p, info.sms);
+        clip_norm_kernel<<<blocks, kThreads, 0, stream>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "clip_norm_kernel");
+        p.n_parts += blocks;
+    }
+    if (p.n_parts == 0) {
+        const cudaError_t e = cudaMemsetAsync(norm, 0, sizeof(float), stream);
+        return e == cudaSuccess ? POLICY_OK : cuda_fail(e, "cudaMemsetAsync");
+    }
+    p.norm = norm;
+    for (int64_t i = 0; i < n;) {
+        i += fill_launch(grads + i, n - i, p);
+        if (p.chunks == 0) continue;
+        clip_scale_kernel<<<launch_blocks(p, info.sms), kThreads, 0, stream>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "clip_scale_kernel");
+        p.norm = nullptr;
+    }
+    return POLICY_OK;
+}
+
+}  // namespace
+}  // namespace policy
+
+using namespace policy;
+
+extern "C" uint64_t policy_clip_grad_workspace_bytes(const policy_grad* grads, int64_t n)
+try {
+    if (check_grads(grads, n) != POLICY_OK) return 0;
+    // one launch for every kTensors non-empty tensors, at most the resident blocks of a full device each
+    const int64_t launches = (n + kTensors - 1) / kTensors + 1;
+    return static_cast<uint64_t>(launches) * kMaxSms * kBlocksPerSm * sizeof(double);
+} catch (...) {
+    return 0;
+}
+
+extern "C" int policy_clip_grad_norm(const policy_grad* grads, int64_t n, float max_norm, float* norm, int device, void* workspace,
+                                     void* stream)
+try {
+    return run_clip(grads, n, max_norm, norm, device, workspace, static_cast<cudaStream_t>(stream));
+} catch (...) {
+    return POLICY_ERR_INVALID;
+}
