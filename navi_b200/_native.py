@@ -7,9 +7,11 @@ loaded, every call that needs it raises RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 from pathlib import Path
+from types import ModuleType
 
 LIB_DIR = Path(__file__).resolve().parent / "_lib"
 # $NAVI_TSDF_DEBUG=1 selects the bounds-checked build (kernel indices checked, a device
@@ -19,12 +21,14 @@ TSDF_PATH = LIB_DIR / ("libnavi_tsdf_debug.so" if os.environ.get("NAVI_TSDF_DEBU
 GMDAG_PATH = LIB_DIR / "libnavi_gmdag.so"
 GMDAG_GPU_PATH = LIB_DIR / "libnavi_gmdag_gpu.so"
 POLICY_PATH = LIB_DIR / "libnavi_policy.so"
+POLICY_TORCH_PATH = LIB_DIR / "navi_policy_torch.so"
 
 _lock = threading.Lock()
 _tsdf: ctypes.CDLL | None = None
 _gmdag: ctypes.CDLL | None = None
 _gmdag_gpu: ctypes.CDLL | None = None
 _policy: ctypes.CDLL | None = None
+_policy_torch: ModuleType | None = None
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -215,18 +219,19 @@ class PolicyGrad(ctypes.Structure):
 POLICY_F32 = 0  # policy_dtype of include/policy.h
 POLICY_BF16 = 1
 
-# name -> (restype, argtypes); mirrors include/policy.h
+# name -> (restype, argtypes); mirrors include/policy.h.  Structures are passed by address
+# (ctypes.byref).
 POLICY_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "policy_version": (c_int, []),
     "policy_last_error": (c_char_p, []),
-    "policy_cross_attention_workspace_bytes": (c_uint64, [ctypes.POINTER(PolicyAttention), c_int]),
-    "policy_cross_attention": (c_int, [ctypes.POINTER(PolicyAttention), c_void_p]),
-    "policy_cross_attention_backward": (c_int, [ctypes.POINTER(PolicyAttention), c_void_p]),
-    "policy_qk_norm_workspace_bytes": (c_uint64, [ctypes.POINTER(PolicyQkNorm)]),
-    "policy_qk_norm_rotary": (c_int, [ctypes.POINTER(PolicyQkNorm), c_void_p]),
-    "policy_qk_norm_rotary_backward": (c_int, [ctypes.POINTER(PolicyQkNorm), c_void_p]),
-    "policy_clip_grad_workspace_bytes": (c_uint64, [ctypes.POINTER(PolicyGrad), c_int64]),
-    "policy_clip_grad_norm": (c_int, [ctypes.POINTER(PolicyGrad), c_int64, c_float, c_void_p, c_int, c_void_p, c_void_p]),
+    "policy_cross_attention_workspace_bytes": (c_uint64, [c_void_p, c_int]),
+    "policy_cross_attention": (c_int, [c_void_p, c_void_p]),
+    "policy_cross_attention_backward": (c_int, [c_void_p, c_void_p]),
+    "policy_qk_norm_workspace_bytes": (c_uint64, [c_void_p]),
+    "policy_qk_norm_rotary": (c_int, [c_void_p, c_void_p]),
+    "policy_qk_norm_rotary_backward": (c_int, [c_void_p, c_void_p]),
+    "policy_clip_grad_workspace_bytes": (c_uint64, [c_void_p, c_int64]),
+    "policy_clip_grad_norm": (c_int, [c_void_p, c_int64, c_float, c_void_p, c_int, c_void_p, c_void_p]),
 }
 
 
@@ -301,10 +306,27 @@ def policy_lib() -> ctypes.CDLL:
     return _policy
 
 
-def check_policy(rc: int, what: str) -> None:
-    if rc != 0:
-        msg = policy_lib().policy_last_error()
-        raise RuntimeError(f"{what} failed ({rc}): {msg.decode() if msg else ''}")
+def policy_torch() -> ModuleType:
+    """The policy operators on torch tensors; raises RuntimeError when the module is not built or cannot load."""
+    global _policy_torch
+    if _policy_torch is None:
+        with _lock:
+            if _policy_torch is None:
+                if not POLICY_TORCH_PATH.exists():
+                    raise RuntimeError(
+                        f"navi_b200 policy operators not found at {POLICY_TORCH_PATH}; run `python -m navi_b200.build`"
+                    )
+                import torch  # noqa: F401  (its libraries resolve the module's symbols)
+
+                name = POLICY_TORCH_PATH.stem
+                spec = importlib.util.spec_from_file_location(name, POLICY_TORCH_PATH)
+                try:
+                    module = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(module)
+                except ImportError as e:
+                    raise RuntimeError(f"navi_b200 policy operators could not be loaded: {e}") from e
+                _policy_torch = module
+    return _policy_torch
 
 
 def last_error() -> str:

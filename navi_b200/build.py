@@ -11,6 +11,7 @@
 - libnavi_gmdag_gpu.so : the device scene compiler (nvcc sm_100a, -fmad=false,
                      IEEE division / sqrt; same words as libnavi_gmdag.so)
 - libnavi_policy.so : the policy operators and the C ABI of include/policy.h (nvcc sm_100a)
+- navi_policy_torch.so : those operators on torch tensors, with their autograd nodes (g++, torch's headers)
 - libnavi_probe.so : the L2 read-bandwidth probe of the benchmark's roofline
 
 All are rebuilt only when a source is newer than the library.
@@ -22,6 +23,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -131,8 +133,33 @@ def build_policy(force: bool = False) -> Path:
         tmp = out.with_suffix(".so.tmp")
         _run([
             _nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-            "-Xcompiler", "-fvisibility=hidden", "-Xlinker", "--exclude-libs,ALL", "--threads", "0",
+            "-Xcompiler", "-fvisibility=hidden", "-Xlinker", "--exclude-libs,ALL", "-Xlinker", f"-soname={out.name}",
+            "--threads", "0",
             f"-I{INCLUDE}", *map(str, srcs), "-o", str(tmp),
+        ])
+        tmp.replace(out)
+    return out
+
+
+def build_policy_torch(force: bool = False) -> Path:
+    """navi_policy_torch.so: the Python module that puts libnavi_policy.so to work on torch tensors."""
+    out = LIB / "navi_policy_torch.so"
+    src = CSRC / "policy_torch.cpp"
+    if force or _stale(out, [src, INCLUDE / "policy.h"]):
+        import torch
+        from torch.utils import cpp_extension
+
+        build_policy()
+        torch_lib = Path(torch.__file__).parent / "lib"
+        cuda = Path(_nvcc()).resolve().parent.parent
+        tmp = out.with_suffix(".so.tmp")
+        _run([
+            host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *(f"-isystem{d}" for d in cpp_extension.include_paths()), f"-I{sysconfig.get_paths()['include']}",
+            f"-I{cuda / 'include'}", f"-I{INCLUDE}", str(src), "-o", str(tmp),
+            f"-L{LIB}", "-lnavi_policy", "-Wl,-rpath,$ORIGIN",
+            f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
         ])
         tmp.replace(out)
     return out
@@ -154,7 +181,7 @@ def build_probe(force: bool = False) -> Path:
 
 def build_all(force: bool = False) -> list[Path]:
     return [build_tsdf(force), build_tsdf(force, bounds_check=True), build_gmdag(force), build_gmdag_gpu(force),
-            build_policy(force), build_probe(force)]
+            build_policy(force), build_policy_torch(force), build_probe(force)]
 
 
 if __name__ == "__main__":

@@ -1,0 +1,87 @@
+// What the cross attention kernels share.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "policy_mma.cuh"
+
+namespace policy {
+
+struct AttnParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* dout;
+    int64_t qs[3], ks[3], vs[3], ds[3];
+    const uint8_t* mask;
+    int64_t mask_stride;
+    const int32_t* lengths;
+    void* out;
+    float* lse;
+    const float* delta;
+    void* dq;
+    void* dk;
+    void* dv;
+    float* part;      // f32 parts of a split launch
+    float* part_ml;   // forward: the parts' (maximum, sum)
+    int64_t q_count;  // values of q, and of k: the parts' strides
+    int64_t k_count;
+    int lq, lk, heads, kv_heads, group, dim, rows;
+    int tiles;        // row tiles (forward, dq) or key tiles (dk, dv) of the grid
+    int splits;
+    float scale, scale_log2;
+};
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;  // relative error below 2^-22; 0 for -inf
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The rows of one (batch, key head): offsets of row r in a strided [batch][lq][heads][dim]
+// tensor and in the contiguous one.
+struct Rows {
+    int64_t b;
+    int hk, group;
+    __device__ __forceinline__ int64_t at(const int64_t (&s)[3], int r) const
+    {
+        const int l = r / group;
+        return b * s[0] + l * s[1] + (static_cast<int64_t>(hk) * group + (r - l * group)) * s[2];
+    }
+    // index of the row in [batch][lq][heads]
+    __device__ __forceinline__ int64_t index(const AttnParams& p, int r) const
+    {
+        const int l = r / group;
+        return (b * p.lq + l) * p.heads + static_cast<int64_t>(hk) * group + (r - l * group);
+    }
+};
+
+__device__ __forceinline__ int visible_keys(const AttnParams& p, int64_t b)
+{
+    if (!p.lengths) return p.lk;
+    return min(max(__ldg(p.lengths + b), 0), p.lk);
+}
+
+// 4 values of a row
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d)
+{
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+template <>
+__device__ __forceinline__ void store4<bf16>(bf16* p, float a, float b, float c, float d)
+{
+    *reinterpret_cast<uint2*>(p) = make_uint2(Mma<bf16>::pack(a, b), Mma<bf16>::pack(c, d));
+}
+
+// The forward on the tensor cores of tcgen05 (policy_attention_tc.cu): bf16, tiles of 256 rows.
+constexpr int kTcRows = 256;
+constexpr int kTcKeys = 128;
+int launch_attend_tc(const AttnParams& p, int64_t bh, int sms, int device, cudaStream_t stream);
+
+}  // namespace policy

@@ -20,7 +20,8 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 4096;        // values: 16 per thread
 constexpr int kBlocksPerSm = 8;     // 256 threads: the SM is full
 constexpr int kMaxSms = 256;         // SMs that the workspace allows for
-constexpr int kTensors = 512;       // tensors of one launch (its parameters)
+constexpr int kTensors = 512;       // tensors of one launch (its parameters: 16 KB)
+constexpr int kFewTensors = 64;     // a launch of up to this many takes 2 KB of parameters instead
 
 struct ClipTensor {
     const void* grad;
@@ -30,8 +31,9 @@ struct ClipTensor {
     uint32_t dtype;        // bit 0: bf16; bit 1: every chunk is 16-byte aligned
 };
 
+template <int N>
 struct ClipParams {
-    ClipTensor t[kTensors];
+    ClipTensor t[N];
     double* parts;
     float* norm;
     float max_norm;
@@ -41,7 +43,8 @@ struct ClipParams {
     int n_parts; // all partial sums (second pass)
 };
 
-__device__ __forceinline__ int find_tensor(const ClipParams& p, uint32_t chunk)
+template <int N>
+__device__ __forceinline__ int find_tensor(const ClipParams<N>& p, uint32_t chunk)
 {
     int lo = 0, hi = p.n - 1;
     while (lo < hi) {
@@ -81,7 +84,8 @@ __device__ __forceinline__ uint32_t scale2(uint32_t w, float c)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_constant__ ClipParams p)
+template <int N>
+__global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_constant__ ClipParams<N> p)
 {
     double sum = 0.0;
     for (uint32_t chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
@@ -126,7 +130,8 @@ __global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_consta
     if (threadIdx.x == 0) p.parts[p.part0 + blockIdx.x] = sum;
 }
 
-__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ ClipParams p)
+template <int N>
+__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ ClipParams<N> p)
 {
     double sum = 0.0;
     for (int i = threadIdx.x; i < p.n_parts; i += kThreads) sum += p.parts[i];
@@ -190,12 +195,13 @@ int check_grads(const policy_grad* grads, int64_t n)
 }
 
 // Takes tensors from grads[i..] for one launch; returns how many entries it consumed.
-int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams& p)
+template <int N>
+int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams<N>& p)
 {
     p.n = 0;
     uint64_t chunks = 0;
     int64_t i = 0;
-    for (; i < n && p.n < kTensors; ++i) {
+    for (; i < n && p.n < N; ++i) {
         const policy_grad& g = grads[i];
         if (g.count == 0) continue;
         const uint64_t own = (g.count + kChunk - 1) / kChunk;
@@ -211,23 +217,17 @@ int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams& p)
     return i;
 }
 
-int launch_blocks(const ClipParams& p, int sms)
+template <int N>
+int launch_blocks(const ClipParams<N>& p, int sms)
 {
     const uint32_t most = static_cast<uint32_t>(sms < kMaxSms ? sms : kMaxSms) * kBlocksPerSm;
     return static_cast<int>(p.chunks < most ? p.chunks : most);
 }
 
-int run_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, int device, void* workspace, cudaStream_t stream)
+template <int N>
+int launch_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, int sms, void* workspace, cudaStream_t stream)
 {
-    int rc = check_grads(grads, n);
-    if (rc != POLICY_OK) return rc;
-    if (!(max_norm >= 0.f)) return fail(POLICY_ERR_INVALID, "max_norm must not be negative");
-    if (!norm) return fail(POLICY_ERR_INVALID, "norm must not be null");
-    const DeviceInfo info = device_info(device);
-    if (info.status != POLICY_OK) return info.status;
-    DeviceScope scope(device);
-    if (scope.error() != cudaSuccess) return cuda_fail(scope.error(), "cudaSetDevice");
-    ClipParams p;
+    ClipParams<N> p;
     p.parts = static_cast<double*>(workspace);
     p.max_norm = max_norm;
     p.n_parts = 0;
@@ -236,7 +236,7 @@ int run_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, i
         if (p.chunks == 0) continue;
         if (!workspace) return fail(POLICY_ERR_INVALID, "workspace must not be null");
         p.part0 = p.n_parts;
-        const int blocks = launch_blocks(p, info.sms);
+        const int blocks = launch_blocks(p, sms);
         clip_norm_kernel<<<blocks, kThreads, 0, stream>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "clip_norm_kernel");
@@ -250,12 +250,26 @@ int run_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, i
     for (int64_t i = 0; i < n;) {
         i += fill_launch(grads + i, n - i, p);
         if (p.chunks == 0) continue;
-        clip_scale_kernel<<<launch_blocks(p, info.sms), kThreads, 0, stream>>>(p);
+        clip_scale_kernel<<<launch_blocks(p, sms), kThreads, 0, stream>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "clip_scale_kernel");
         p.norm = nullptr;
     }
     return POLICY_OK;
+}
+
+int run_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, int device, void* workspace, cudaStream_t stream)
+{
+    const int rc = check_grads(grads, n);
+    if (rc != POLICY_OK) return rc;
+    if (!(max_norm >= 0.f)) return fail(POLICY_ERR_INVALID, "max_norm must not be negative");
+    if (!norm) return fail(POLICY_ERR_INVALID, "norm must not be null");
+    const DeviceInfo info = device_info(device);
+    if (info.status != POLICY_OK) return info.status;
+    DeviceScope scope(device);
+    if (scope.error() != cudaSuccess) return cuda_fail(scope.error(), "cudaSetDevice");
+    if (n <= kFewTensors) return launch_clip<kFewTensors>(grads, n, max_norm, norm, info.sms, workspace, stream);
+    return launch_clip<kTensors>(grads, n, max_norm, norm, info.sms, workspace, stream);
 }
 
 }  // namespace

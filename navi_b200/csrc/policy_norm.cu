@@ -3,12 +3,17 @@
 //   u = w x r,  r = 1 / sqrt(mean(x^2) + eps);   y = R u, R the rotation of the first values
 // and, since R is orthogonal,
 //   g = R^T dy,  dw = sum over rows of g x r,  dx = r w g - r^3 x mean(w g x).
-// Memory bounds both: one read of x (and dy) and one write.  A row belongs to dim / 8 neighbouring
+// Memory bounds both: one read of x (and dy) and one write.  A row belongs to LANES neighbouring
 // lanes with 8 values each, so that a rotation's partner values sit rotary / 16 lanes away and are
-// shuffled, not read again; a thread takes up to four heads of one token, which share the token's
-// cosines and sines.  Everything between the read and the one rounding at the store is in 32 bits.
+// shuffled, not read again.  A thread keeps one token and up to HEADS of its heads and walks over
+// batches: without positions the token's cosines and sines (four times the bytes of a bfloat16
+// value each) are read once for all of them, and the next batch's rows are read while this one's
+// are worked on.  Everything between the read and the one rounding at the store is in 32 bits, two
+// values to an instruction (the f32x2 forms), since at 16 bits a value the issue slots come next
+// after memory.
 #include <cuda_bf16.h>
 
+#include <cmath>
 #include <limits>
 
 #include "policy_internal.h"
@@ -18,7 +23,6 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;  // heads of a token per thread
 
 struct NormSide {
     const void* x;
@@ -29,224 +33,315 @@ struct NormSide {
     const int32_t* positions;
     int64_t xs[3], ds[3];
     int64_t table_rows;
-    int64_t units;      // (batch, token, group of kHeads heads)
     float* part;        // backward: [blocks][dim], null without dweight
     float* dweight;
-    int tokens, heads, chunks;
+    int tokens, heads;
+    int chunks;         // groups of HEADS heads
+    int splits;         // batch ranges
     int blocks;
 };
 
 struct NormParams {
     NormSide side[2];
-    int dim, rotary, lanes;  // lanes per row, a power of two
-    float eps;
+    int batch, dim, rotary;
+    float eps, inv_dim;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p);
-template <>
-__device__ __forceinline__ void load8<float>(float (&v)[8], const float* p)
+// two f32 values in a register pair
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float a, float b)
 {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
-template <>
-__device__ __forceinline__ void load8<bf16>(float (&v)[8], const bf16* p)
+__device__ __forceinline__ float2 both(F2 v)
 {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]);
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8])
+__device__ __forceinline__ F2 mul2(F2 a, F2 b)
 {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
-template <>
-__device__ __forceinline__ void store8<bf16>(bf16* p, const float (&v)[8])
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
 {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 shuffle2(F2 v, int lane)
+{
+    const float2 f = both(v);
+    return pair(__shfl_sync(0xffffffffu, f.x, lane), __shfl_sync(0xffffffffu, f.y, lane));
 }
 
-__device__ __forceinline__ float row_sum(float x, int lanes)
+// 8 values as they lie in memory
+template <typename T>
+struct Raw;
+template <>
+struct Raw<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p)
+    {
+        a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    }
+    __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void get(F2 (&v)[4]) const
+    {
+        v[0] = pair(a.x, a.y), v[1] = pair(a.z, a.w), v[2] = pair(b.x, b.y), v[3] = pair(b.z, b.w);
+    }
+    static __device__ __forceinline__ void store(float* p, const F2 (&v)[4])
+    {
+        const float2 x = both(v[0]), y = both(v[1]), z = both(v[2]), w = both(v[3]);
+        *reinterpret_cast<float4*>(p) = make_float4(x.x, x.y, y.x, y.y);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(z.x, z.y, w.x, w.y);
+    }
+};
+template <>
+struct Raw<bf16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void clear() { a = make_uint4(0u, 0u, 0u, 0u); }
+    static __device__ __forceinline__ F2 one(uint32_t w)
+    {
+        return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    __device__ __forceinline__ void get(F2 (&v)[4]) const { v[0] = one(a.x), v[1] = one(a.y), v[2] = one(a.z), v[3] = one(a.w); }
+    static __device__ __forceinline__ void store(bf16* p, const F2 (&v)[4])
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = both(v[i]);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+template <int LANES>
+__device__ __forceinline__ float row_sum(F2 x)
 {
-    for (int d = 1; d < lanes; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    return x;
+    const float2 f = both(x);
+    float s = f.x + f.y;
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    return s;
 }
 
-// A lane's place in its row and the token it works on.
-struct Place {
-    int sub;            // lane of the row
-    int pair;           // lane that holds the rotation's other value, or this one
-    bool in_dim, low;   // low: the first half of a rotated pair
-    __device__ __forceinline__ Place(const NormParams& p)
+// What a thread works on: its lane of the row, its token and heads, and its range of batches.
+template <int LANES, int HEADS>
+struct Work {
+    int sub;              // lane of the row
+    int other;            // lane that holds the rotation's other value, or this one
+    bool low, turned;     // in the first half of a rotated pair, in either
+    bool active;
+    int token, h0, heads; // heads of this thread that exist
+    int b0, b1;
+    __device__ __forceinline__ Work(const NormParams& p, const NormSide& s, int block)
     {
         const int lane = threadIdx.x & 31, half = p.rotary / 16;
-        sub = lane & (p.lanes - 1);
-        in_dim = sub * 8 < p.dim;
+        sub = lane & (LANES - 1);
         low = sub < half;
-        pair = low ? lane + half : sub < 2 * half ? lane - half : lane;
+        turned = sub < 2 * half;
+        other = low ? lane + half : turned ? lane - half : lane;
+        const int64_t unit = static_cast<int64_t>(block) * (kThreads / LANES) + threadIdx.x / LANES;
+        const int64_t row = unit / s.chunks;
+        h0 = static_cast<int>(unit - row * s.chunks) * HEADS;
+        const int split = static_cast<int>(row / s.tokens);
+        token = static_cast<int>(row - static_cast<int64_t>(split) * s.tokens);
+        active = split < s.splits && sub * 8 < p.dim;
+        heads = active ? min(HEADS, s.heads - h0) : 0;
+        // every lane of a warp takes part in the shuffles of as many rounds as the longest range has
+        b0 = split < s.splits ? static_cast<int>(static_cast<int64_t>(p.batch) * split / s.splits) : 0;
+        b1 = split < s.splits ? static_cast<int>(static_cast<int64_t>(p.batch) * (split + 1) / s.splits) : 0;
     }
 };
 
-// The cosines and signed sines of a lane's 8 values: y = u cos + other sin.  Returns false for a
-// position outside the table.
-__device__ __forceinline__ bool angles(const NormParams& p, const NormSide& s, const Place& at, int64_t b, int token, bool active,
-                                       float (&cs)[8], float (&sn)[8])
+// The cosines and signed sines of a lane's 8 values, y = u cos + other sin; false for a position
+// outside the table.
+template <int LANES, int HEADS>
+__device__ __forceinline__ bool angles(const NormParams& p, const NormSide& s, const Work<LANES, HEADS>& at, int64_t pos, F2 (&cs)[4],
+                                       F2 (&sn)[4])
 {
-    const int half = p.rotary / 16;
-    int64_t pos = token;
-    if (s.positions && active) pos = s.positions[b * s.tokens + token];
     const bool inside = pos >= 0 && pos < s.table_rows;
-    if (active && inside && at.sub < 2 * half) {
-        const float* row = s.table + pos * p.rotary + (at.low ? at.sub : at.sub - half) * 8;
-        load8(cs, row);
-        load8(sn, row + p.rotary / 2);
-        if (at.low) {
+    if (at.active && inside && at.turned) {
+        const float* row = s.table + pos * p.rotary + (at.low ? at.sub : at.sub - p.rotary / 16) * 8;
+        Raw<float> c, n;
+        c.load(row);
+        n.load(row + p.rotary / 2);
+        c.get(cs);
+        n.get(sn);
+        const float sign = at.low ? -1.f : 1.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
-        }
+        for (int i = 0; i < 4; ++i) sn[i] = mul2(sn[i], pair(sign, sign));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+        for (int i = 0; i < 4; ++i) cs[i] = pair(1.f, 1.f), sn[i] = pair(0.f, 0.f);
     }
     return inside;
 }
 
-template <typename T>
+__device__ __forceinline__ void load_weight(F2 (&w)[4], const NormSide& s, int sub, bool active)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pair(1.f, 1.f);
+    if (s.weight && active) {
+        Raw<float> r;
+        r.load(s.weight + sub * 8);
+        r.get(w);
+    }
+}
+
+template <typename T, int LANES, int HEADS>
 __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant__ NormParams p)
 {
     const bool second = blockIdx.x >= p.side[0].blocks;
     const NormSide& s = p.side[second ? 1 : 0];
-    const int block = second ? blockIdx.x - p.side[0].blocks : blockIdx.x;
-    const Place at(p);
-    const int rows = kThreads / p.lanes;
-    float w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 1.f;
-    if (s.weight && at.in_dim) load8(w, s.weight + at.sub * 8);
+    const Work<LANES, HEADS> at(p, s, second ? blockIdx.x - p.side[0].blocks : blockIdx.x);
+    F2 w[4], cs[4], sn[4];
+    load_weight(w, s, at.sub, at.active);
+    bool inside = true;
+    if (s.table && !s.positions) inside = angles(p, s, at, at.token, cs, sn);
 
-    for (int64_t base = static_cast<int64_t>(block) * rows; base < s.units; base += static_cast<int64_t>(s.blocks) * rows) {
-        const int64_t unit = base + threadIdx.x / p.lanes;
-        const bool active = unit < s.units && at.in_dim;
-        const int64_t bt = unit < s.units ? unit / s.chunks : 0;
-        const int h0 = unit < s.units ? static_cast<int>(unit - bt * s.chunks) * kHeads : 0;
-        const int64_t b = bt / s.tokens;
-        const int token = static_cast<int>(bt - b * s.tokens);
-        const T* x = static_cast<const T*>(s.x) + b * s.xs[0] + token * s.xs[1] + h0 * s.xs[2] + at.sub * 8;
-        T* y = static_cast<T*>(s.y) + (bt * s.heads + h0) * p.dim + at.sub * 8;
-        float v[kHeads][8];
+    const int rounds = __reduce_max_sync(0xffffffffu, at.b1 - at.b0);
+    const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
+    T* y = static_cast<T*>(s.y) + ((static_cast<int64_t>(at.b0) * s.tokens + at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
+    const int64_t y_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
+    Raw<T> next[HEADS];
+    int64_t next_pos = 0;
+    auto fetch = [&](int i) {
+        const bool on = at.b0 + i < at.b1;
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[h][i] = 0.f;
-            if (active && h0 + h < s.heads) load8(v[h], x + h * s.xs[2]);
+        for (int h = 0; h < HEADS; ++h) {
+            if (on && h < at.heads) next[h].load(x + i * s.xs[0] + h * s.xs[2]);
+            else next[h].clear();
         }
-        float cs[8], sn[8];
-        bool inside = true;
-        if (s.table) inside = angles(p, s, at, b, token, active, cs, sn);
+        if (s.positions && on) next_pos = s.positions[static_cast<int64_t>(at.b0 + i) * s.tokens + at.token];
+    };
+    fetch(0);
+    for (int i = 0; i < rounds; ++i) {
+        F2 v[HEADS][4];
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-            float sum = 0.f;
+        for (int h = 0; h < HEADS; ++h) next[h].get(v[h]);
+        const int64_t pos = next_pos;
+        if (i + 1 < rounds) fetch(i + 1);
+        if (s.positions) inside = angles(p, s, at, pos, cs, sn);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(v[h][i], v[h][i], sum);
-            const float r = rsqrtf(row_sum(sum, p.lanes) / p.dim + p.eps);
+        for (int h = 0; h < HEADS; ++h) {
+            F2 sum = mul2(v[h][0], v[h][0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[h][i] = v[h][i] * r * w[i];
+            for (int k = 1; k < 4; ++k) sum = fma2(v[h][k], v[h][k], sum);
+            const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
+            const F2 r2 = pair(r, r);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[h][k] = mul2(mul2(v[h][k], r2), w[k]);
             if (s.table) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float other = __shfl_sync(0xffffffffu, v[h][i], at.pair);
-                    v[h][i] = inside ? fmaf(v[h][i], cs[i], other * sn[i]) : NAN;
+                for (int k = 0; k < 4; ++k) {
+                    const F2 o = shuffle2(v[h][k], at.other);
+                    v[h][k] = fma2(v[h][k], cs[k], mul2(o, sn[k]));
+                    if (!inside) v[h][k] = pair(NAN, NAN);
                 }
             }
-            if (active && h0 + h < s.heads) store8(y + h * p.dim, v[h]);
+            if (h < at.heads && at.b0 + i < at.b1) Raw<T>::store(y + h * p.dim, v[h]);
         }
+        y += y_step;
     }
 }
 
-template <typename T>
+template <typename T, int LANES, int HEADS>
 __global__ void __launch_bounds__(kThreads) qk_norm_grad_kernel(const __grid_constant__ NormParams p)
 {
     __shared__ float sums[kThreads * 8];
     const bool second = blockIdx.x >= p.side[0].blocks;
     const NormSide& s = p.side[second ? 1 : 0];
     const int block = second ? blockIdx.x - p.side[0].blocks : blockIdx.x;
-    const Place at(p);
-    const int rows = kThreads / p.lanes;
-    float w[8], dw[8];
+    const Work<LANES, HEADS> at(p, s, block);
+    F2 w[4], dw[4], cs[4], sn[4];
+    load_weight(w, s, at.sub, at.active);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 1.f, dw[i] = 0.f;
-    if (s.weight && at.in_dim) load8(w, s.weight + at.sub * 8);
+    for (int k = 0; k < 4; ++k) dw[k] = pair(0.f, 0.f);
+    bool inside = true;
+    if (s.table && !s.positions) inside = angles(p, s, at, at.token, cs, sn);
 
-    for (int64_t base = static_cast<int64_t>(block) * rows; base < s.units; base += static_cast<int64_t>(s.blocks) * rows) {
-        const int64_t unit = base + threadIdx.x / p.lanes;
-        const bool active = unit < s.units && at.in_dim;
-        const int64_t bt = unit < s.units ? unit / s.chunks : 0;
-        const int h0 = unit < s.units ? static_cast<int>(unit - bt * s.chunks) * kHeads : 0;
-        const int64_t b = bt / s.tokens;
-        const int token = static_cast<int>(bt - b * s.tokens);
-        const T* x = static_cast<const T*>(s.x) + b * s.xs[0] + token * s.xs[1] + h0 * s.xs[2] + at.sub * 8;
-        const T* dy = static_cast<const T*>(s.dy) + b * s.ds[0] + token * s.ds[1] + h0 * s.ds[2] + at.sub * 8;
-        T* dx = static_cast<T*>(s.y) + (bt * s.heads + h0) * p.dim + at.sub * 8;
-        float cs[8], sn[8];
-        bool inside = true;
-        if (s.table) inside = angles(p, s, at, b, token, active, cs, sn);
+    const int rounds = __reduce_max_sync(0xffffffffu, at.b1 - at.b0);
+    const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
+    const T* dy = static_cast<const T*>(s.dy) + at.b0 * s.ds[0] + at.token * s.ds[1] + at.h0 * s.ds[2] + at.sub * 8;
+    T* dx = static_cast<T*>(s.y) + ((static_cast<int64_t>(at.b0) * s.tokens + at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
+    const int64_t dx_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
+    for (int i = 0; i < rounds; ++i) {
+        const bool on = at.b0 + i < at.b1;
+        Raw<T> rx[HEADS], rg[HEADS];
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-            const bool on = active && h0 + h < s.heads;
-            float v[8], g[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = g[i] = 0.f;
-            if (on) {
-                load8(v, x + h * s.xs[2]);
-                load8(g, dy + h * s.ds[2]);
+        for (int h = 0; h < HEADS; ++h) {
+            if (on && h < at.heads) {
+                rx[h].load(x + i * s.xs[0] + h * s.xs[2]);
+                rg[h].load(dy + i * s.ds[0] + h * s.ds[2]);
+            } else {
+                rx[h].clear();
+                rg[h].clear();
             }
+        }
+        if (s.positions) {
+            int64_t pos = at.token;
+            if (on) pos = s.positions[static_cast<int64_t>(at.b0 + i) * s.tokens + at.token];
+            inside = angles(p, s, at, pos, cs, sn);
+        }
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            const bool here = on && h < at.heads;
+            F2 v[4], g[4];
+            rx[h].get(v);
+            rg[h].get(g);
             if (s.table) {  // the rotation back: the sines change sign
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float other = __shfl_sync(0xffffffffu, g[i], at.pair);
-                    g[i] = inside ? fmaf(g[i], cs[i], -other * sn[i]) : on ? NAN : 0.f;
+                for (int k = 0; k < 4; ++k) {
+                    const F2 o = shuffle2(g[k], at.other);
+                    g[k] = fma2(g[k], cs[k], mul2(mul2(o, sn[k]), pair(-1.f, -1.f)));
+                    if (!inside && here) g[k] = pair(NAN, NAN);
                 }
             }
-            float sum = 0.f, dot = 0.f;
+            F2 sum = mul2(v[0], v[0]), dot = mul2(mul2(v[0], w[0]), g[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sum = fmaf(v[i], v[i], sum);
-                dot = fmaf(v[i] * w[i], g[i], dot);
+            for (int k = 1; k < 4; ++k) {
+                sum = fma2(v[k], v[k], sum);
+                dot = fma2(mul2(v[k], w[k]), g[k], dot);
             }
-            const float r = rsqrtf(row_sum(sum, p.lanes) / p.dim + p.eps);
-            const float f = r * r * r * (row_sum(dot, p.lanes) / p.dim);
+            const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
+            const float f = -r * r * r * (row_sum<LANES>(dot) * p.inv_dim);
+            const F2 r2 = pair(r, r), f2 = pair(f, f);
+            if (here) {
+                F2 d[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (on) dw[i] = fmaf(g[i], v[i] * r, dw[i]);
-                v[i] = fmaf(r * w[i], g[i], -f * v[i]);
+                for (int k = 0; k < 4; ++k) {
+                    const F2 gr = mul2(g[k], r2);
+                    dw[k] = fma2(gr, v[k], dw[k]);
+                    d[k] = fma2(gr, w[k], mul2(f2, v[k]));
+                }
+                Raw<T>::store(dx + h * p.dim, d);
             }
-            if (on) store8(dx + h * p.dim, v);
         }
+        dx += dx_step;
     }
     if (!s.part) return;
     // the block's rows, in order
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[(threadIdx.x / p.lanes) * p.lanes * 8 + at.sub * 8 + i] = dw[i];
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = both(dw[k]);
+        float* at_row = sums + (threadIdx.x / LANES) * (LANES * 8) + at.sub * 8 + 2 * k;
+        at_row[0] = f.x, at_row[1] = f.y;
+    }
     __syncthreads();
     for (int d = threadIdx.x; d < p.dim; d += kThreads) {
-        float x = 0.f;
-        for (int r = 0; r < rows; ++r) x += sums[r * p.lanes * 8 + d];
-        s.part[static_cast<int64_t>(block) * p.dim + d] = x;
+        float t = 0.f;
+        for (int r = 0; r < kThreads / LANES; ++r) t += sums[r * (LANES * 8) + d];
+        s.part[static_cast<int64_t>(block) * p.dim + d] = t;
     }
 }
 
@@ -317,36 +412,78 @@ int check_norm_pointers(const policy_qk_norm* a, bool backward)
     return POLICY_OK;
 }
 
-// Blocks of each side: enough to fill the device several times over; at most one per group of rows.
-constexpr int kBlocksPerSm = 8;
+// Lanes of a row and heads of a thread.  A wider group than the dim needs leaves lanes idle, so the
+// lanes follow the dim; the heads follow the side with more rows (heads that a side does not have
+// are not worked on).
+struct NormShape {
+    int lanes, heads;
+};
 
-NormParams make_norm(const policy_qk_norm& a, int sms, bool backward)
+NormShape norm_shape(const policy_qk_norm& a)
 {
-    NormParams p{};
-    p.dim = a.dim, p.rotary = a.rotary, p.eps = a.eps;
-    p.lanes = 1;
-    while (p.lanes * 8 < a.dim) p.lanes *= 2;
-    const int rows = kThreads / p.lanes;
+    NormShape s{4, 4};
+    while (s.lanes * 8 < a.dim) s.lanes *= 2;
+    const policy_norm_side& big = a.side[0].tokens * a.side[0].heads > a.side[1].tokens * a.side[1].heads ? a.side[0] : a.side[1];
+    if (big.heads <= 2) s.heads = big.heads;
+    return s;
+}
+
+// Threads' ranges of batches: as long as they leave the device kRounds full sets of blocks.
+constexpr int kBlocksPerSm = 8;
+constexpr int kRounds = 2;
+
+int make_norm(const policy_qk_norm& a, int sms, bool backward, NormParams& p)
+{
+    p = NormParams{};
+    const NormShape shape = norm_shape(a);
+    p.batch = static_cast<int>(a.batch), p.dim = a.dim, p.rotary = a.rotary, p.eps = a.eps;
+    p.inv_dim = 1.f / static_cast<float>(a.dim);
+    const int64_t groups = kThreads / shape.lanes;
     int64_t total = 0;
     for (int i = 0; i < 2; ++i) {
         const policy_norm_side& s = a.side[i];
         NormSide& d = p.side[i];
         d.x = s.x, d.dy = s.dy, d.y = backward ? s.dx : s.y;
-        d.weight = s.weight, d.table = a.rotary ? s.table : nullptr, d.positions = s.positions;
+        d.weight = s.weight, d.table = a.rotary ? s.table : nullptr, d.positions = a.rotary ? s.positions : nullptr;
         for (int k = 0; k < 3; ++k) d.xs[k] = s.strides[k], d.ds[k] = s.dy_strides[k];
         d.table_rows = s.table_rows;
         d.tokens = static_cast<int>(s.tokens), d.heads = s.heads;
-        d.chunks = (s.heads + kHeads - 1) / kHeads;
-        d.units = a.batch * s.tokens * d.chunks;
-        total += d.units;
+        d.chunks = (s.heads + shape.heads - 1) / shape.heads;
+        total += a.batch * s.tokens * d.chunks;
     }
+    const int64_t want = static_cast<int64_t>(sms) * kBlocksPerSm * kRounds * groups;
+    const int64_t length = total / want > 1 ? total / want : 1;  // batches of a thread
     for (NormSide& d : p.side) {
-        const int64_t most = (d.units + rows - 1) / rows;
-        // a side's share of the resident blocks, by its rows
-        int64_t share = total ? (static_cast<int64_t>(sms) * kBlocksPerSm * d.units + total - 1) / total : 0;
-        d.blocks = static_cast<int>(share < most ? share : most);
+        d.splits = static_cast<int>((a.batch + length - 1) / length);
+        const int64_t blocks = (static_cast<int64_t>(d.splits) * d.tokens * d.chunks + groups - 1) / groups;
+        if (blocks > kMaxInt / 2) return fail(POLICY_ERR_INVALID, "the launch would need over 2^30 blocks");
+        d.blocks = static_cast<int>(blocks);
     }
-    return p;
+    return POLICY_OK;
+}
+
+template <typename T, int LANES, int HEADS>
+void launch_norm(const NormParams& p, bool backward, unsigned blocks, cudaStream_t stream)
+{
+    if (backward) qk_norm_grad_kernel<T, LANES, HEADS><<<blocks, kThreads, 0, stream>>>(p);
+    else qk_norm_kernel<T, LANES, HEADS><<<blocks, kThreads, 0, stream>>>(p);
+}
+
+template <typename T, int LANES>
+void launch_norm(const NormParams& p, int heads, bool backward, unsigned blocks, cudaStream_t stream)
+{
+    if (heads == 1) launch_norm<T, LANES, 1>(p, backward, blocks, stream);
+    else if (heads == 2) launch_norm<T, LANES, 2>(p, backward, blocks, stream);
+    else launch_norm<T, LANES, 4>(p, backward, blocks, stream);
+}
+
+template <typename T>
+void launch_norm(const NormParams& p, const NormShape& s, bool backward, unsigned blocks, cudaStream_t stream)
+{
+    if (s.lanes == 4) launch_norm<T, 4>(p, s.heads, backward, blocks, stream);
+    else if (s.lanes == 8) launch_norm<T, 8>(p, s.heads, backward, blocks, stream);
+    else if (s.lanes == 16) launch_norm<T, 16>(p, s.heads, backward, blocks, stream);
+    else launch_norm<T, 32>(p, s.heads, backward, blocks, stream);
 }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -359,8 +496,9 @@ int run_norm(const policy_qk_norm* a, bool backward, cudaStream_t stream)
     if (info.status != POLICY_OK) return info.status;
     DeviceScope scope(a->device);
     if (scope.error() != cudaSuccess) return cuda_fail(scope.error(), "cudaSetDevice");
-    NormParams p = make_norm(*a, info.sms, backward);
-    const int blocks = p.side[0].blocks + p.side[1].blocks;
+    NormParams p;
+    if ((rc = make_norm(*a, info.sms, backward, p)) != POLICY_OK) return rc;
+    const unsigned blocks = static_cast<unsigned>(p.side[0].blocks) + static_cast<unsigned>(p.side[1].blocks);
     bool weights = false;
     if (backward) {
         char* ws = static_cast<char*>(a->workspace);
@@ -374,15 +512,10 @@ int run_norm(const policy_qk_norm* a, bool backward, cudaStream_t stream)
             weights = true;
         }
     }
-    const bool f32 = a->dtype == POLICY_F32;
     if (blocks > 0) {
-        if (!backward) {
-            if (f32) qk_norm_kernel<float><<<blocks, kThreads, 0, stream>>>(p);
-            else qk_norm_kernel<bf16><<<blocks, kThreads, 0, stream>>>(p);
-        } else {
-            if (f32) qk_norm_grad_kernel<float><<<blocks, kThreads, 0, stream>>>(p);
-            else qk_norm_grad_kernel<bf16><<<blocks, kThreads, 0, stream>>>(p);
-        }
+        const NormShape shape = norm_shape(*a);
+        if (a->dtype == POLICY_F32) launch_norm<float>(p, shape, backward, blocks, stream);
+        else launch_norm<bf16>(p, shape, backward, blocks, stream);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "qk_norm_kernel");
     }
@@ -404,7 +537,8 @@ try {
     if (check_norm(a) != POLICY_OK) return 0;
     const DeviceInfo info = device_info(a->device);
     if (info.status != POLICY_OK) return 0;
-    const NormParams p = make_norm(*a, info.sms, true);
+    NormParams p;
+    if (make_norm(*a, info.sms, true, p) != POLICY_OK) return 0;
     return align256(sizeof(float) * p.side[0].blocks * p.dim) + align256(sizeof(float) * p.side[1].blocks * p.dim);
 } catch (...) {
     return 0;

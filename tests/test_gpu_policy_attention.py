@@ -270,6 +270,15 @@ def test_captured_in_a_graph():
     ref.assert_close(out, ref.attention(q, k, v, visible), ref.FORWARD[torch.bfloat16], "out")
 
 
+def test_gradients_of_gradients_are_an_error():
+    q, k, v, do, _, _ = inputs((1, 2, 9, 2, 2, 32), torch.float32)
+    q.requires_grad_()
+    out = policy.cross_attention(q, k, v)
+    (dq,) = torch.autograd.grad(out, q, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="once only"):
+        dq.sum().backward()
+
+
 def test_refusals():
     q, k, v, _, _, _ = inputs((2, 3, 10, 4, 2, 32), torch.float32)
     bad = [

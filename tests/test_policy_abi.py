@@ -59,7 +59,7 @@ def _attention(**kw) -> _native.PolicyAttention:
 ])
 def test_attention_refuses(change, text):
     lib = _native.policy_lib()
-    assert lib.policy_cross_attention(_attention(**change), None) == -1
+    assert lib.policy_cross_attention(ctypes.byref(_attention(**change)), None) == -1
     assert text in lib.policy_last_error().decode()
 
 
@@ -70,7 +70,7 @@ def test_attention_refuses(change, text):
 def test_attention_backward_refuses(change, text):
     lib = _native.policy_lib()
     a = _attention(q=16, k=16, v=16, out=16, **change)
-    assert lib.policy_cross_attention_backward(a, None) == -1
+    assert lib.policy_cross_attention_backward(ctypes.byref(a), None) == -1
     assert text in lib.policy_last_error().decode()
 
 
@@ -97,7 +97,7 @@ def test_norm_refuses(change, text):
         s.tokens, s.heads = 1, 1
     for n, v in change.items():
         setattr(a, n, v)
-    assert lib.policy_qk_norm_rotary(a, None) == -1
+    assert lib.policy_qk_norm_rotary(ctypes.byref(a), None) == -1
     assert text in lib.policy_last_error().decode()
 
 
