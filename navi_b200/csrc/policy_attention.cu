@@ -946,7 +946,8 @@ AttnParams make_params(const policy_attention& a)
 // How a call is laid out: tiles, splits and workspace, from the sizes alone.
 struct Plan {
     int dp = 0;              // padded head dimension: 32, 64 or 128
-    int fwd_rows = 0;        // rows of a forward tile: 16, 32 or 64
+    bool tc = false;         // forward on tcgen05
+    int fwd_rows = 0;        // rows of a forward tile: 16, 32 or 64, or 256 with tcgen05
     int fwd_keys = 0;
     int fwd_splits = 1;
     bool few = false;        // gradients in one kernel
@@ -960,9 +961,9 @@ size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // Blocks to aim at, as blocks per SM that a launch of this kind keeps resident; a split below two
 // tiles would cost more in parts than it gives.
-int choose_splits(int64_t blocks, int tiles, int sms)
+int choose_splits(int64_t blocks, int tiles, int sms, int per_sm = 4)
 {
-    const int64_t want = (static_cast<int64_t>(sms) * 4 + blocks - 1) / (blocks > 0 ? blocks : 1);
+    const int64_t want = (static_cast<int64_t>(sms) * per_sm + blocks - 1) / (blocks > 0 ? blocks : 1);
     const int64_t most = tiles / 2 > 1 ? tiles / 2 : 1;
     return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
 }
@@ -977,10 +978,12 @@ Plan make_plan(const policy_attention& a, int sms)
     pl.fwd_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     if (f32) pl.fwd_keys = pl.dp == 128 ? 32 : 64;
     else pl.fwd_keys = pl.dp == 128 || pl.fwd_rows == 64 ? 64 : 128;
+    pl.tc = !f32 && rows > 64;
+    if (pl.tc) pl.fwd_rows = kTcRows, pl.fwd_keys = kTcKeys;
     pl.grad_warps = f32 && pl.dp == 128 ? 2 : 4;
     const int64_t q_count = a.batch * a.lq * a.heads * a.dim, k_count = a.batch * a.lk * a.kv_heads * a.dim;
     if (bh == 0) return pl;
-    pl.fwd_splits = choose_splits(bh * ceil_div(rows, pl.fwd_rows), ceil_div(a.lk, pl.fwd_keys), sms);
+    pl.fwd_splits = choose_splits(bh * ceil_div(rows, pl.fwd_rows), ceil_div(a.lk, pl.fwd_keys), sms, pl.tc ? 1 : 4);
     if (pl.fwd_splits > 1)
         pl.fwd_bytes = align256(sizeof(float) * pl.fwd_splits * q_count) + align256(sizeof(float) * 2 * pl.fwd_splits * (q_count / a.dim));
     pl.few = rows <= 16;
@@ -1054,7 +1057,7 @@ int launch_fwd_rows(const AttnParams& p, const Plan& pl, int64_t bh, int device,
 }
 
 template <typename T>
-int run_forward(const policy_attention& a, const Plan& pl, cudaStream_t stream)
+int run_forward(const policy_attention& a, const Plan& pl, int sms, cudaStream_t stream)
 {
     AttnParams p = make_params(a);
     const int64_t bh = a.batch * a.kv_heads;
@@ -1064,7 +1067,8 @@ int run_forward(const policy_attention& a, const Plan& pl, cudaStream_t stream)
         p.part = static_cast<float*>(a.workspace);
         p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + align256(sizeof(float) * p.splits * p.q_count));
     }
-    int rc = pl.dp == 32   ? launch_fwd_rows<T, 32>(p, pl, bh, a.device, stream)
+    int rc = pl.tc         ? launch_attend_tc(p, bh, sms, a.device, stream)
+             : pl.dp == 32 ? launch_fwd_rows<T, 32>(p, pl, bh, a.device, stream)
              : pl.dp == 64 ? launch_fwd_rows<T, 64>(p, pl, bh, a.device, stream)
                            : launch_fwd_rows<T, 128>(p, pl, bh, a.device, stream);
     if (rc != POLICY_OK || p.splits == 1) return rc;
@@ -1161,7 +1165,7 @@ int forward(const policy_attention& a, int sms, cudaStream_t stream)
     if (a.lk == 0) return zero<T>(a.out, rows * a.dim, a.lse, rows, stream);
     const Plan pl = make_plan(a, sms);
     if (pl.fwd_bytes && !a.workspace) return fail(POLICY_ERR_INVALID, "workspace must not be null");
-    return run_forward<T>(a, pl, stream);
+    return run_forward<T>(a, pl, sms, stream);
 }
 
 template <typename T>
