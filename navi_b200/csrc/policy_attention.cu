@@ -978,7 +978,7 @@ Plan make_plan(const policy_attention& a, int sms)
     pl.fwd_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     if (f32) pl.fwd_keys = pl.dp == 128 ? 32 : 64;
     else pl.fwd_keys = pl.dp == 128 || pl.fwd_rows == 64 ? 64 : 128;
-    pl.tc = !f32 && rows > 64;
+    pl.tc = !f32 && rows > 64 && attend_tc_takes(make_params(a));
     if (pl.tc) pl.fwd_rows = kTcRows, pl.fwd_keys = kTcKeys;
     pl.grad_warps = f32 && pl.dp == 128 ? 2 : 4;
     const int64_t q_count = a.batch * a.lq * a.heads * a.dim, k_count = a.batch * a.lk * a.kv_heads * a.dim;

@@ -82,6 +82,9 @@ __device__ __forceinline__ void store4<bf16>(bf16* p, float a, float b, float c,
 // The forward on the tensor cores of tcgen05 (policy_attention_tc.cu): bf16, tiles of 256 rows.
 constexpr int kTcRows = 256;
 constexpr int kTcKeys = 128;
+// Whether the strides of k and v fit the copies' descriptors: below 2^40 bytes, and keys that are not all
+// the same one.
+bool attend_tc_takes(const AttnParams& p);
 int launch_attend_tc(const AttnParams& p, int64_t bh, int sms, int device, cudaStream_t stream);
 
 }  // namespace policy

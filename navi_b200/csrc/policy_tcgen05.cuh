@@ -17,14 +17,26 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
+// One arrival for a warp whose lanes have all come here (arrivals on one barrier are served one by one).
+__device__ __forceinline__ void warp_arrive(uint32_t bar)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(bar);
+}
+// One arrival, after which the phase also waits for `bytes` of copies.
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Whether the phase is over; the hardware may hold the thread for up to some microseconds until it is.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
 {
     uint32_t done;
     asm volatile(
         "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
         "selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        : "=r"(done) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
     return done != 0;
 }
 __device__ __forceinline__ uint64_t nanoseconds()
@@ -43,8 +55,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     if (bar_try(bar, parity)) return true;
     const uint64_t start = nanoseconds();
     for (;;) {
-        for (int i = 0; i < 32; ++i)
-            if (bar_try(bar, parity)) return true;
+        if (bar_try(bar, parity)) return true;
         if (*broken) return false;
         if (nanoseconds() - start > kWaitLimit) {
             *broken = 1;
@@ -123,13 +134,14 @@ constexpr uint32_t kBlockRow = 128;  // bytes
 
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * kBlockRow + ((piece ^ (row & 7)) << 4); }
 
-// The matrix descriptor of a swizzled tile.  `next_block`: bytes from one 64-column block to the next, used
-// where the blocks run along the product's M or N; rows advance 8 at a time by 1,024 bytes.
-__device__ __forceinline__ uint64_t tile_descriptor(uint32_t addr, uint32_t next_block)
+// The matrix descriptor of a swizzled tile.  Its low word holds the address and `next_block`, the bytes from one
+// 64-column block to the next, used where the blocks run along the product's M or N; its high word says that
+// rows advance 8 at a time by 1,024 bytes.  Advancing the address adds its sixteenth to the low word.
+__device__ __forceinline__ uint32_t tile_descriptor(uint32_t addr, uint32_t next_block)
 {
-    return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | static_cast<uint64_t>(next_block >> 4) << 16 |
-           static_cast<uint64_t>(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
+    return ((addr & 0x3ffffu) >> 4) | (next_block >> 4) << 16;
 }
+constexpr uint32_t kDescriptorHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
 
 // bf16 x bf16 -> f32, M x N; transposed_x: the operand is stored with its M (or N) axis contiguous.
 __host__ __device__ constexpr uint32_t bf16_product(int m, int n, bool transposed_a, bool transposed_b)
@@ -138,21 +150,34 @@ __host__ __device__ constexpr uint32_t bf16_product(int m, int n, bool transpose
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
 }
 
-// d (+)= a b, 16 deep, both operands in shared memory.  One thread issues all products of a block, which
+// One lane of a converged warp.  The compiler knows that one lane at most goes on; under a plain test of the lane
+// it would have to issue the products, whose operands sit in the warp's uniform registers, in a loop over lanes.
+__device__ __forceinline__ bool elected()
+{
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
+}
+
+// d (+)= a b, 16 deep, both operands in shared memory.  One elected thread issues all products of a block, which
 // the tensor core runs in the order of issue.
-__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add)
+__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t kind, bool add)
 {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+        "{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.u32 p, %4, 0;\n"
+        "mov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(kind), "r"(static_cast<uint32_t>(add)),
+        "n"(kDescriptorHigh)
         : "memory");
 }
 // the same with a in tensor memory: two bf16 of a row in each column
-__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add)
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t kind, bool add)
 {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+        "{\n.reg .pred p;\n.reg .b64 y;\nsetp.ne.u32 p, %4, 0;\n"
+        "mov.b64 y, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(kind), "r"(static_cast<uint32_t>(add)),
+        "n"(kDescriptorHigh)
         : "memory");
 }
 // One arrival at `bar` when every product issued so far by the calling thread is complete.
