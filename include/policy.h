@@ -58,8 +58,12 @@ POLICY_API const char* policy_last_error(void);
  *
  * dim is a multiple of 8, 8 to 128.  q, k, v and dout have element stride 1 along dim,
  * 16-byte aligned rows (base address, and strides times the element size).  out, dq, dk
- * and dv are contiguous; lse is [batch][lq][heads] f32, in base 2 (log2 of the sum of
- * exp(s_ij)), +inf for a query that gives 0.  Forward: lse may be null.  Backward: out and lse are the forward's. */
+ * and dv are contiguous; For the backward pass the
+ * forward writes, where the pointers are not null, stats [batch][lq][heads][2] f32 (the exponent that its
+ * weights are relative to, in base 2, and the reciprocal of their sum, 0 for a query that gives 0: a single
+ * logarithm of the sum would carry its own rounding into every weight), and with POLICY_BF16 out_rest, bf16 in
+ * the layout of out: what the rounding of out left off (dout . out in 8 bits would be the largest error of dq
+ * and dk where a query sees few keys; null in the backward: taken as 0). */
 typedef struct policy_attention {
     int32_t device;
     int32_t dtype;
@@ -76,7 +80,8 @@ typedef struct policy_attention {
     int64_t key_mask_stride;
     const int32_t* key_lengths;
     void* out;
-    float* lse;
+    float* stats;
+    void* out_rest;
     /* backward only */
     const void* dout;
     int64_t dout_strides[3];

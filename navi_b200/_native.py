@@ -183,7 +183,7 @@ class PolicyAttention(ctypes.Structure):
         ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
         ("q_strides", Strides), ("k_strides", Strides), ("v_strides", Strides),
         ("key_mask", c_void_p), ("key_mask_stride", c_int64), ("key_lengths", c_void_p),
-        ("out", c_void_p), ("lse", c_void_p),
+        ("out", c_void_p), ("stats", c_void_p), ("out_rest", c_void_p),
         ("dout", c_void_p), ("dout_strides", Strides),
         ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
         ("workspace", c_void_p),

@@ -9,7 +9,7 @@
 // with c = scale log2(e).  Rows beyond the last and keys that are not visible are zeros in
 // shared memory, so nothing that masked keys hold reaches a product.
 //
-// Gradient: p_ij = 2^(c s_ij - lse_i), D_i = do_i . o_i, ds_ij = p_ij (do_i . v_j - D_i);
+// Gradient: p_ij = 2^(c s_ij - x_i) y_i (the forward's reference exponent and reciprocal sum), D_i = do_i . o_i, ds_ij = p_ij (do_i . v_j - D_i);
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j.
 // Up to 16 rows one kernel reads each key and value once and makes all three gradients; with
 // more rows one kernel makes dk and dv (a key tile stays, rows stream), one dq (rows stay,
@@ -302,8 +302,8 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
         const int64_t row = rows.index(p, r0 + r);
         if (p.splits == 1) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            store4(static_cast<T*>(p.out) + row * p.dim + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-            if (d == 0 && p.lse) p.lse[row] = l == 0.f ? INFINITY : base + log2f(l);
+            store_out<T>(p, row * p.dim + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            if (d == 0 && p.stats) p.stats[row] = row_stats(base, l);
         } else {
             store4(p.part + split * p.q_count + row * p.dim + d, x.x, x.y, x.z, x.w);
             if (d == 0) {
@@ -338,15 +338,15 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttnParams p)
         x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    store4(static_cast<T*>(p.out) + row * p.dim + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-    if (d == 0 && p.lse) p.lse[row] = l == 0.f ? INFINITY : base + log2f(l);
+    store_out<T>(p, row * p.dim + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    if (d == 0 && p.stats) p.stats[row] = row_stats(base, l);
 }
 
 // --- gradients -----------------------------------------------------------------
 
-// D_i = do_i . o_i of every row: 8 lanes to a row.
+// D_i = do_i . o_i of a row, b and its rest (or null) together being o: 8 lanes to a row.
 template <typename T>
-__device__ __forceinline__ float row_dot(const T* a, const T* b, int dim, int sub)
+__device__ __forceinline__ float row_dot(const T* a, const T* b, const T* rest, int dim, int sub)
 {
     float x = 0.f;
     for (int d = sub * 4; d < dim; d += 32) {
@@ -360,6 +360,12 @@ __device__ __forceinline__ float row_dot(const T* a, const T* b, int dim, int su
             const float2 w0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
             const float2 w1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
             x = fmaf(u0.x, w0.x, fmaf(u0.y, w0.y, fmaf(u1.x, w1.x, fmaf(u1.y, w1.y, x))));
+            if (rest) {
+                const uint2 z = *reinterpret_cast<const uint2*>(rest + d);
+                const float2 z0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&z.x));
+                const float2 z1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&z.y));
+                x = fmaf(u0.x, z0.x, fmaf(u0.y, z0.y, fmaf(u1.x, z1.x, fmaf(u1.y, z1.y, x))));
+            }
         }
     }
     x += __shfl_xor_sync(0xffffffffu, x, 1);
@@ -376,7 +382,8 @@ __global__ void __launch_bounds__(256) attend_delta_kernel(const AttnParams p, f
     const int h = static_cast<int>(row % p.heads);
     const int64_t bl = row / p.heads, b = bl / p.lq, l = bl - b * p.lq;
     const T* g = static_cast<const T*>(p.dout) + b * p.ds[0] + l * p.ds[1] + h * p.ds[2];
-    const float x = row_dot(g, static_cast<const T*>(p.out) + row * p.dim, p.dim, threadIdx.x & 7);
+    const T* rest = p.rest ? static_cast<const T*>(p.rest) + row * p.dim : nullptr;
+    const float x = row_dot(g, static_cast<const T*>(p.out) + row * p.dim, rest, p.dim, threadIdx.x & 7);
     if (i < n_rows && (threadIdx.x & 7) == 0) delta[row] = x;
 }
 
@@ -389,12 +396,12 @@ struct GradShape {
     static constexpr int OPITCH = DP + 4;
     static constexpr size_t kKeys = sizeof(T) * KT * PITCH;
     // all gradients, 16 rows
-    static constexpr size_t kFewStream = 4 * kKeys + sizeof(T) * (2 * 16 * PITCH + NW * 16 * TP) + 2 * KT + 128;
+    static constexpr size_t kFewStream = 4 * kKeys + sizeof(T) * (2 * 16 * PITCH + NW * 16 * TP) + 2 * KT + 16 * 3 * sizeof(float);
     static constexpr size_t kMerge = sizeof(float) * NW * 16 * OPITCH;
     static constexpr size_t kFew = kFewStream > kMerge ? kFewStream : kMerge;
     // dk and dv: RT rows stream
     static constexpr int RT = 32;
-    static constexpr size_t kKeyGrad = 2 * kKeys + 4 * sizeof(T) * RT * PITCH + 4 * RT * sizeof(float) + KT;
+    static constexpr size_t kKeyGrad = 2 * kKeys + 4 * sizeof(T) * RT * PITCH + 6 * RT * sizeof(float) + KT;
     // dq: 16 NW rows stay, QT keys stream
     static constexpr int QT = 32;
     static constexpr size_t kQueryStream = 2 * kKeys + 4 * sizeof(T) * QT * PITCH + 2 * QT;
@@ -428,8 +435,8 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
     T* sq = sv + 2 * KT * PITCH;
     T* sdo = sq + 16 * PITCH;
     T* str = sdo + 16 * PITCH;
-    float* slse = reinterpret_cast<float*>(str + NW * 16 * S::TP);
-    float* sdelta = slse + 16;
+    float2* sstats = reinterpret_cast<float2*>(str + NW * 16 * S::TP);
+    float* sdelta = reinterpret_cast<float*>(sstats + 16);
     uint8_t* svis = reinterpret_cast<uint8_t*>(sdelta + 16);
 
     const int split = blockIdx.x % p.splits;
@@ -437,6 +444,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
     const Rows rows{bh / p.kv_heads, bh % p.kv_heads, p.group};
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = visible_keys(p, rows.b);
+    const bool single = n == 1;  // the softmax of one score is constant: its gradient is 0, not a rounding of it
     const int tiles = (p.lk + KT - 1) / KT;
     const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / p.splits);
     const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / p.splits);
@@ -451,9 +459,9 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
         const int rr = min(r, p.rows - 1);
         const int64_t row = rows.index(p, rr);
         const float x = row_dot(static_cast<const T*>(p.dout) + rows.at(p.ds, rr), static_cast<const T*>(p.out) + row * p.dim,
-                                p.dim, threadIdx.x & 7);
+                                p.rest ? static_cast<const T*>(p.rest) + row * p.dim : nullptr, p.dim, threadIdx.x & 7);
         if ((threadIdx.x & 7) == 0) {
-            slse[r] = r < p.rows ? p.lse[row] : INFINITY;
+            sstats[r] = r < p.rows ? p.stats[row] : make_float2(0.f, 0.f);
             sdelta[r] = r < p.rows ? x : 0.f;
         }
     }
@@ -500,10 +508,11 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = j * 8 + (lane & 3) * 2 + (i & 1);
-                const bool on = (i < 2 ? on0 : on1) && slse[r] != INFINITY;
-                const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -slse[r]));
+                const float2 st_r = sstats[r];
+                const bool on = (i < 2 ? on0 : on1) && st_r.y != 0.f;
+                const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -st_r.x)) * st_r.y;
                 s[j][i] = on ? w : 0.f;
-                dp[j][i] = on ? w * (dp[j][i] - sdelta[r]) : 0.f;
+                dp[j][i] = on && !single ? w * (dp[j][i] - sdelta[r]) : 0.f;
                 const int key = (lane >> 2) + (i < 2 ? 0 : 8);
                 if constexpr (sizeof(T) == 2) tr[r * S::TP + key] = __float2bfloat16_rn(dp[j][i]);
                 else tr[r * S::TP + key] = dp[j][i];
@@ -589,8 +598,8 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
     T* sv = sk + KT * PITCH;
     T* sq = sv + KT * PITCH;
     T* sdo = sq + 2 * RT * PITCH;
-    float* slse = reinterpret_cast<float*>(sdo + 2 * RT * PITCH);
-    float* sdelta = slse + 2 * RT;
+    float2* sstats = reinterpret_cast<float2*>(sdo + 2 * RT * PITCH);
+    float* sdelta = reinterpret_cast<float*>(sstats + 2 * RT);
     uint8_t* svis = reinterpret_cast<uint8_t*>(sdelta + 2 * RT);
 
     const int split = blockIdx.x % p.splits;
@@ -599,6 +608,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
     const Rows rows{bh / p.kv_heads, bh % p.kv_heads, p.group};
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = visible_keys(p, rows.b);
+    const bool single = n == 1;
     const int row_tiles = (p.rows + RT - 1) / RT;
     const int t0 = static_cast<int>(static_cast<int64_t>(row_tiles) * split / p.splits);
     const int t1 = static_cast<int>(static_cast<int64_t>(row_tiles) * (split + 1) / p.splits);
@@ -608,12 +618,13 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
     auto issue = [&](int t, int st) {
         load_rows<T, DP, PITCH, RT, S::THREADS>(sq + st * RT * PITCH, static_cast<const T*>(p.q), p.qs, rows, t * RT, p.rows, p.dim);
         load_rows<T, DP, PITCH, RT, S::THREADS>(sdo + st * RT * PITCH, static_cast<const T*>(p.dout), p.ds, rows, t * RT, p.rows, p.dim);
-        for (int i = threadIdx.x; i < 2 * RT; i += S::THREADS) {
-            const int r = t * RT + (i & (RT - 1));
-            const float* src = i < RT ? p.lse : p.delta;
+        for (int i = threadIdx.x; i < RT; i += S::THREADS) {
+            const int r = t * RT + i;
             const bool take = r < p.rows;
-            const uint32_t dst = smem_addr((i < RT ? slse : sdelta) + st * RT + (i & (RT - 1)));
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(take ? src + rows.index(p, r) : src),
+            const int64_t row = take ? rows.index(p, r) : 0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_addr(sstats + st * RT + i)), "l"(p.stats + row),
+                         "r"(take ? 8 : 0) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_addr(sdelta + st * RT + i)), "l"(p.delta + row),
                          "r"(take ? 4 : 0) : "memory");
         }
     };
@@ -660,11 +671,11 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = j * 8 + (lane & 3) * 2 + (i & 1);
-                const float lse = slse[st * RT + r];
-                const bool on = (i < 2 ? on0 : on1) && lse != INFINITY;
-                const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -lse));
+                const float2 st_r = sstats[st * RT + r];
+                const bool on = (i < 2 ? on0 : on1) && st_r.y != 0.f;
+                const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -st_r.x)) * st_r.y;
                 s[j][i] = on ? w : 0.f;
-                dp[j][i] = on ? w * (dp[j][i] - sdelta[st * RT + r]) : 0.f;
+                dp[j][i] = on && !single ? w * (dp[j][i] - sdelta[st * RT + r]) : 0.f;
             }
         }
         typename M::A pf[RS], df[RS];
@@ -754,12 +765,13 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
         if (t0 + 1 < t1) bits = loader.visible((t0 + 1) * KT);
     }
     copy_commit();
-    float lse[2], delta[2];
+    float2 stats[2];
+    float delta[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = r0 + warp * 16 + (lane >> 2) + 8 * h;
         const int64_t row = rows.index(p, min(r, p.rows - 1));
-        lse[h] = r < p.rows ? p.lse[row] : INFINITY;
+        stats[h] = r < p.rows && n > 1 ? p.stats[row] : make_float2(0.f, 0.f);  // one visible key: no gradient
         delta[h] = r < p.rows ? p.delta[row] : 0.f;
     }
     float dq[DP / 8][4];
@@ -803,8 +815,8 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int h = i >> 1;
-                const bool on = ((i & 1) ? vis.y : vis.x) && lse[h] != INFINITY;
-                const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -lse[h]));
+                const bool on = ((i & 1) ? vis.y : vis.x) && stats[h].y != 0.f;
+                const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -stats[h].x)) * stats[h].y;
                 dp[j][i] = on ? w * (dp[j][i] - delta[h]) : 0.f;
             }
         }
@@ -856,11 +868,12 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, int64
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) zero_kernel(T* out, int64_t count, float* lse, int64_t rows)
+__global__ void __launch_bounds__(256) zero_kernel(T* out, T* rest, int64_t count, float2* stats, int64_t rows)
 {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i * 4 < count) store4(out + i * 4, 0.f, 0.f, 0.f, 0.f);
-    if (lse && i < rows) lse[i] = INFINITY;
+    if (rest && i * 4 < count) store4(rest + i * 4, 0.f, 0.f, 0.f, 0.f);
+    if (stats && i < rows) stats[i] = make_float2(0.f, 0.f);
 }
 
 // --- host ----------------------------------------------------------------------
@@ -907,6 +920,8 @@ int check_args(const policy_attention* a, bool backward)
     if (a->lq > 0) {
         if ((rc = check_strides("q", a->q, a->q_strides, e)) != POLICY_OK) return rc;
         if ((rc = check_output("out", a->out)) != POLICY_OK) return rc;
+        if (a->stats && (rc = check_output("stats", a->stats)) != POLICY_OK) return rc;
+        if (a->out_rest && (rc = check_output("out_rest", a->out_rest)) != POLICY_OK) return rc;
     }
     if (a->lk > 0) {
         if ((rc = check_strides("k", a->k, a->k_strides, e)) != POLICY_OK) return rc;
@@ -915,7 +930,7 @@ int check_args(const policy_attention* a, bool backward)
     if (!backward) return POLICY_OK;
     if (a->lq > 0) {
         if ((rc = check_strides("dout", a->dout, a->dout_strides, e)) != POLICY_OK) return rc;
-        if (!a->lse) return fail(POLICY_ERR_INVALID, "lse must not be null");
+        if ((rc = check_output("stats", a->stats)) != POLICY_OK) return rc;
         if ((rc = check_output("dq", a->dq)) != POLICY_OK) return rc;
     }
     if (a->lk > 0) {
@@ -931,7 +946,7 @@ AttnParams make_params(const policy_attention& a)
     p.q = a.q, p.k = a.k, p.v = a.v, p.dout = a.dout;
     for (int i = 0; i < 3; ++i) p.qs[i] = a.q_strides[i], p.ks[i] = a.k_strides[i], p.vs[i] = a.v_strides[i], p.ds[i] = a.dout_strides[i];
     p.mask = a.key_mask, p.mask_stride = a.key_mask_stride, p.lengths = a.key_lengths;
-    p.out = a.out, p.lse = a.lse, p.dq = a.dq, p.dk = a.dk, p.dv = a.dv;
+    p.out = a.out, p.rest = a.dtype == POLICY_BF16 ? a.out_rest : nullptr, p.stats = reinterpret_cast<float2*>(a.stats), p.dq = a.dq, p.dk = a.dk, p.dv = a.dv;
     p.q_count = a.batch * a.lq * a.heads * a.dim;
     p.k_count = a.batch * a.lk * a.kv_heads * a.dim;
     p.lq = static_cast<int>(a.lq), p.lk = static_cast<int>(a.lk);
@@ -1146,14 +1161,14 @@ int run_backward_dim(const policy_attention& a, const Plan& pl, cudaStream_t str
 }
 
 template <typename T>
-int zero(void* out, int64_t count, float* lse, int64_t rows, cudaStream_t stream)
+int zero(void* out, void* rest, int64_t count, float* stats, int64_t rows, cudaStream_t stream)
 {
     const int64_t n = count / 4 > rows ? count / 4 : rows;
     if (n == 0) return POLICY_OK;
     unsigned grid = 0;
     const int rc = launch_blocks((n + 255) / 256, "policy_cross_attention", grid);
     if (rc != POLICY_OK) return rc;
-    zero_kernel<T><<<grid, 256, 0, stream>>>(static_cast<T*>(out), count, lse, rows);
+    zero_kernel<T><<<grid, 256, 0, stream>>>(static_cast<T*>(out), static_cast<T*>(rest), count, reinterpret_cast<float2*>(stats), rows);
     return launched("zero_kernel");
 }
 
@@ -1162,7 +1177,7 @@ int forward(const policy_attention& a, int sms, cudaStream_t stream)
 {
     const int64_t rows = a.batch * a.lq * a.heads;
     if (rows == 0) return POLICY_OK;
-    if (a.lk == 0) return zero<T>(a.out, rows * a.dim, a.lse, rows, stream);
+    if (a.lk == 0) return zero<T>(a.out, a.out_rest, rows * a.dim, a.stats, rows, stream);
     const Plan pl = make_plan(a, sms);
     if (pl.fwd_bytes && !a.workspace) return fail(POLICY_ERR_INVALID, "workspace must not be null");
     return run_forward<T>(a, pl, sms, stream);
@@ -1174,10 +1189,10 @@ int backward(const policy_attention& a, int sms, cudaStream_t stream)
     if (a.batch == 0) return POLICY_OK;
     const int64_t k_count = a.batch * a.lk * a.kv_heads * a.dim;
     if (a.lq == 0) {
-        const int rc = zero<T>(a.dk, k_count, nullptr, 0, stream);
-        return rc != POLICY_OK ? rc : zero<T>(a.dv, k_count, nullptr, 0, stream);
+        const int rc = zero<T>(a.dk, nullptr, k_count, nullptr, 0, stream);
+        return rc != POLICY_OK ? rc : zero<T>(a.dv, nullptr, k_count, nullptr, 0, stream);
     }
-    if (a.lk == 0) return zero<T>(a.dq, a.batch * a.lq * a.heads * a.dim, nullptr, 0, stream);
+    if (a.lk == 0) return zero<T>(a.dq, nullptr, a.batch * a.lq * a.heads * a.dim, nullptr, 0, stream);
     const Plan pl = make_plan(a, sms);
     if (pl.grad_bytes && !a.workspace) return fail(POLICY_ERR_INVALID, "workspace must not be null");
     if (pl.dp == 32) return run_backward_dim<T, 32, 4>(a, pl, stream);

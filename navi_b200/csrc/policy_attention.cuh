@@ -19,7 +19,8 @@ struct AttnParams {
     int64_t mask_stride;
     const int32_t* lengths;
     void* out;
-    float* lse;
+    float2* stats;    // of a row: exponent of reference, 1 / sum (0: no visible key)
+    void* rest;       // bf16: what the rounding of out left off
     const float* delta;
     void* dq;
     void* dk;
@@ -65,6 +66,8 @@ __device__ __forceinline__ int visible_keys(const AttnParams& p, int64_t b)
     return min(max(__ldg(p.lengths + b), 0), p.lk);
 }
 
+__device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+
 // 4 values of a row
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
@@ -77,6 +80,23 @@ template <>
 __device__ __forceinline__ void store4<bf16>(bf16* p, float a, float b, float c, float d)
 {
     *reinterpret_cast<uint2*>(p) = make_uint2(Mma<bf16>::pack(a, b), Mma<bf16>::pack(c, d));
+}
+
+// 4 values of an output, and what their rounding leaves off where that is wanted
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnParams& p, int64_t at, float a, float b, float c, float d)
+{
+    store4(static_cast<T*>(p.out) + at, a, b, c, d);
+    if constexpr (sizeof(T) == 2) {
+        if (p.rest)
+            store4(static_cast<T*>(p.rest) + at, a - round_bf16(a), b - round_bf16(b), c - round_bf16(c), d - round_bf16(d));
+    }
+}
+
+// A row's weights are 2^(c s - x) y.
+__device__ __forceinline__ float2 row_stats(float reference, float sum)
+{
+    return make_float2(reference, sum == 0.f ? 0.f : 1.f / sum);
 }
 
 // The forward on the tensor cores of tcgen05 (policy_attention_tc.cu): bf16, tiles of 256 rows.

@@ -502,23 +502,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (p.splits == 1) {
                     // through shared memory, so that 8 lanes write a row's 128 bytes: a thread's own row would be 16
                     // bytes in each of 32 places at a time
-                    __syncwarp();
+                    const auto put = [&](void* tensor) {
+                        __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t w[4];
+                        for (int j = 0; j < 8; ++j) {
+                            uint32_t w[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = Mma<bf16>::pack(o[j * 8 + 2 * k] * inv, o[j * 8 + 2 * k + 1] * inv);
-                        *reinterpret_cast<uint4*>(store + swizzled(lane, j)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    __syncwarp();
-                    const int col = q * 64 + (lane & 7) * 8;
+                            for (int k = 0; k < 4; ++k) w[k] = Mma<bf16>::pack(o[j * 8 + 2 * k], o[j * 8 + 2 * k + 1]);
+                            *reinterpret_cast<uint4*>(store + swizzled(lane, j)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        __syncwarp();
+                        const int col = q * 64 + (lane & 7) * 8;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int from = j * 4 + (lane >> 3);
-                        const int64_t to_row = __shfl_sync(0xffffffffu, row, from);
-                        const uint4 w = *reinterpret_cast<const uint4*>(store + swizzled(from, lane & 7));
-                        if (r - lane + from < p.rows && col < p.dim)
-                            *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + to_row * p.dim + col) = w;
+                        for (int j = 0; j < 8; ++j) {
+                            const int from = j * 4 + (lane >> 3);
+                            const int64_t to_row = __shfl_sync(0xffffffffu, row, from);
+                            const uint4 w = *reinterpret_cast<const uint4*>(store + swizzled(from, lane & 7));
+                            if (r - lane + from < p.rows && col < p.dim)
+                                *reinterpret_cast<uint4*>(static_cast<bf16*>(tensor) + to_row * p.dim + col) = w;
+                        }
+                    };
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) o[j] *= inv;
+                    put(p.out);
+                    if (p.rest) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) o[j] -= round_bf16(o[j]);
+                        put(p.rest);
                     }
                 } else if (in) {
                     float* g = p.part + item.split * p.q_count + row * p.dim + q * 64;
@@ -533,8 +543,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (p.splits > 1) {
                 float* ml = p.part_ml + 2 * (item.split * (p.q_count / p.dim) + row);
                 ml[0] = m, ml[1] = ok ? l : NAN;
-            } else if (p.lse) {
-                p.lse[row] = !ok ? NAN : l == 0.f ? INFINITY : (m == -INFINITY ? 0.f : m * c) + log2f(l);
+            } else if (p.stats) {
+                p.stats[row] = ok ? row_stats(m == -INFINITY ? 0.f : m * c, l) : same(NAN);
             }
         }
     }

@@ -110,14 +110,16 @@ policy_attention attention_args(const Tensor& q, const Tensor& k, const Tensor& 
 }
 
 Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& key_mask, const Tensor& key_lengths, double scale,
-              Tensor* lse)
+              Tensor* stats, Tensor* rest)
 {
     Tensor out = at::empty(q.sizes(), q.options());
     policy_attention a = attention_args(q, k, v, key_mask, key_lengths, scale);
     a.out = out.data_ptr();
-    if (lse) {
-        *lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
-        a.lse = lse->data_ptr<float>();
+    if (stats) {  // for the backward pass
+        *stats = at::empty({q.size(0), q.size(1), q.size(2), 2}, q.options().dtype(at::kFloat));
+        a.stats = stats->data_ptr<float>();
+        if (a.dtype == POLICY_BF16) *rest = at::empty(q.sizes(), q.options());
+        a.out_rest = data(*rest);
     }
     const Tensor ws = scratch(policy_cross_attention_workspace_bytes(&a, 0), q);
     a.workspace = data(ws);
@@ -131,21 +133,22 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     {
         const Tensor key_mask = mask.value_or(Tensor()), key_lengths = lengths.value_or(Tensor());
         const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
-        Tensor lse;
-        Tensor out = attend(q, k, v, key_mask, key_lengths, scale, &lse);
-        ctx->save_for_backward({q, k, v, key_mask, key_lengths, out, lse});
+        Tensor stats, rest;
+        Tensor out = attend(q, k, v, key_mask, key_lengths, scale, &stats, &rest);
+        ctx->save_for_backward({q, k, v, key_mask, key_lengths, out, stats, rest});
         ctx->saved_data["scale"] = scale;
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[5], &lse = s[6];
+        const Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[5], &stats = s[6], &rest = s[7];
         const Tensor dout = rows(grads[0].detach());
         policy_attention a = attention_args(q, k, v, s[3], s[4], ctx->saved_data["scale"].toDouble());
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
         a.out = out.data_ptr();
-        a.lse = lse.data_ptr<float>();
+        a.stats = stats.data_ptr<float>();
+        a.out_rest = data(rest);
         a.dout = dout.const_data_ptr();
         put_strides(a.dout_strides, dout);
         a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv = dv.data_ptr();
@@ -185,7 +188,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
         return CrossAttention::apply(q, k, v, optional(key_mask), optional(key_lengths), scale);
     at::NoGradGuard no_grad;
-    return attend(rows(q), rows(k), rows(v), key_mask, key_lengths, scale, nullptr);
+    return attend(rows(q), rows(k), rows(v), key_mask, key_lengths, scale, nullptr, nullptr);
 }
 
 // --- norms of queries and keys with rotation -------------------------------------

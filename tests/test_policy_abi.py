@@ -64,8 +64,8 @@ def test_attention_refuses(change, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    ({}, "dout must not be null"), ({"dout": 16}, "lse must not be null"), ({"dout": 16, "lse": 16}, "dq must not be null"),
-    ({"dout": 16, "lse": 16, "dq": 16}, "dk must not be null"), ({"dout": 16, "lse": 16, "dq": 16, "dk": 16}, "dv must not be null"),
+    ({}, "dout must not be null"), ({"dout": 16}, "stats must not be null"), ({"dout": 16, "stats": 16}, "dq must not be null"),
+    ({"dout": 16, "stats": 16, "dq": 16}, "dk must not be null"), ({"dout": 16, "stats": 16, "dq": 16, "dk": 16}, "dv must not be null"),
 ])
 def test_attention_backward_refuses(change, text):
     lib = _native.policy_lib()
