@@ -126,9 +126,10 @@ def build_gmdag_gpu(force: bool = False) -> Path:
 def build_policy(force: bool = False) -> Path:
     """libnavi_policy.so: cross attention, norms of queries and keys with rotation, gradient clipping."""
     out = LIB / "libnavi_policy.so"
-    srcs = [CSRC / "policy_attention.cu", CSRC / "policy_attention_tc.cu", CSRC / "policy_norm.cu", CSRC / "policy_clip.cu", CSRC / "policy_common.cpp"]
+    srcs = [CSRC / "policy_attention.cu", CSRC / "policy_attention_tc.cu", CSRC / "policy_attention_grad_tc.cu", CSRC / "policy_norm.cu",
+            CSRC / "policy_clip.cu", CSRC / "policy_common.cpp"]
     deps = srcs + [CSRC / "policy_internal.h", CSRC / "policy_attention.cuh", CSRC / "policy_mma.cuh", CSRC / "policy_tcgen05.cuh",
-                   INCLUDE / "policy.h"]
+                   CSRC / "policy_map.h", INCLUDE / "policy.h"]
     if force or _stale(out, deps):
         LIB.mkdir(parents=True, exist_ok=True)
         tmp = out.with_suffix(".so.tmp")

@@ -966,6 +966,7 @@ struct Plan {
     int fwd_keys = 0;
     int fwd_splits = 1;
     bool few = false;        // gradients in one kernel
+    bool grad_tc = false;    // gradients on tcgen05
     int grad_warps = 0;
     int few_splits = 1, key_splits = 1, query_splits = 1;
     size_t fwd_bytes = 0, grad_bytes = 0;
@@ -982,6 +983,9 @@ int choose_splits(int64_t blocks, int tiles, int sms, int per_sm = 4)
     const int64_t most = tiles / 2 > 1 ? tiles / 2 : 1;
     return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
 }
+
+// From this many rows on the gradients run on tcgen05.
+constexpr int kTcGradRows = 64;
 
 Plan make_plan(const policy_attention& a, int sms)
 {
@@ -1008,8 +1012,14 @@ Plan make_plan(const policy_attention& a, int sms)
         if (pl.few_splits > 1) pl.grad_bytes = align256(sizeof(float) * pl.few_splits * q_count);
     } else {
         pl.grad_bytes = align256(sizeof(float) * (q_count / a.dim));
-        pl.key_splits = choose_splits(bh * ceil_div(a.lk, kt), ceil_div(rows, 32), sms);
-        pl.query_splits = choose_splits(bh * ceil_div(rows, kt), ceil_div(a.lk, 32), sms);
+        pl.grad_tc = !f32 && rows > kTcGradRows && attend_grad_tc_takes(make_params(a));
+        if (pl.grad_tc) {
+            pl.key_splits = choose_splits(bh * ceil_div(a.lk, grad_tc_tile(true, a.dim)), ceil_div(rows, kGradTcStream), sms, 2);
+            pl.query_splits = choose_splits(bh * ceil_div(rows, grad_tc_tile(false, a.dim)), ceil_div(a.lk, kGradTcStream), sms, 1);
+        } else {
+            pl.key_splits = choose_splits(bh * ceil_div(a.lk, kt), ceil_div(rows, 32), sms);
+            pl.query_splits = choose_splits(bh * ceil_div(rows, kt), ceil_div(a.lk, 32), sms);
+        }
         if (pl.key_splits > 1) pl.grad_bytes += align256(sizeof(float) * 2 * pl.key_splits * k_count);
         if (pl.query_splits > 1) pl.grad_bytes += align256(sizeof(float) * pl.query_splits * q_count);
     }
@@ -1116,7 +1126,7 @@ int add_parts(const float* part, int64_t stride, int splits, int64_t count, void
 }
 
 template <typename T, int DP, int NW>
-int run_backward_dim(const policy_attention& a, const Plan& pl, cudaStream_t stream)
+int run_backward_dim(const policy_attention& a, const Plan& pl, int sms, cudaStream_t stream)
 {
     using S = GradShape<T, DP, NW>;
     static std::atomic<uint64_t> done_few{0}, done_keys{0}, done_queries{0};
@@ -1141,9 +1151,10 @@ int run_backward_dim(const policy_attention& a, const Plan& pl, cudaStream_t str
     p.delta = delta;
 
     p.splits = pl.key_splits;
-    p.tiles = ceil_div(p.lk, S::KT);
+    p.tiles = ceil_div(p.lk, pl.grad_tc ? grad_tc_tile(true, p.dim) : S::KT);
     p.part = reinterpret_cast<float*>(ws);
-    rc = launch_grad<T>(attend_grad_keys_kernel<T, DP, NW>, S::kKeyGrad, done_keys, p, bh * p.tiles * p.splits, S::THREADS, a.device,
+    if (pl.grad_tc) rc = launch_attend_grad_tc(p, true, bh, sms, a.device, stream);
+    else rc = launch_grad<T>(attend_grad_keys_kernel<T, DP, NW>, S::kKeyGrad, done_keys, p, bh * p.tiles * p.splits, S::THREADS, a.device,
                         stream, "attend_grad_keys_kernel");
     if (rc != POLICY_OK) return rc;
     if (p.splits > 1) {
@@ -1152,9 +1163,10 @@ int run_backward_dim(const policy_attention& a, const Plan& pl, cudaStream_t str
         ws += align256(sizeof(float) * 2 * p.splits * p.k_count);
     }
     p.splits = pl.query_splits;
-    p.tiles = ceil_div(p.rows, NW * 16);
+    p.tiles = ceil_div(p.rows, pl.grad_tc ? grad_tc_tile(false, p.dim) : NW * 16);
     p.part = reinterpret_cast<float*>(ws);
-    rc = launch_grad<T>(attend_grad_queries_kernel<T, DP, NW>, S::kQueryGrad, done_queries, p, bh * p.tiles * p.splits, S::THREADS,
+    if (pl.grad_tc) rc = launch_attend_grad_tc(p, false, bh, sms, a.device, stream);
+    else rc = launch_grad<T>(attend_grad_queries_kernel<T, DP, NW>, S::kQueryGrad, done_queries, p, bh * p.tiles * p.splits, S::THREADS,
                         a.device, stream, "attend_grad_queries_kernel");
     if (rc == POLICY_OK && p.splits > 1) rc = add_parts<T>(p.part, p.q_count, p.splits, p.q_count, p.dq, stream);
     return rc;
@@ -1195,9 +1207,9 @@ int backward(const policy_attention& a, int sms, cudaStream_t stream)
     if (a.lk == 0) return zero<T>(a.dq, nullptr, a.batch * a.lq * a.heads * a.dim, nullptr, 0, stream);
     const Plan pl = make_plan(a, sms);
     if (pl.grad_bytes && !a.workspace) return fail(POLICY_ERR_INVALID, "workspace must not be null");
-    if (pl.dp == 32) return run_backward_dim<T, 32, 4>(a, pl, stream);
-    if (pl.dp == 64) return run_backward_dim<T, 64, 4>(a, pl, stream);
-    return run_backward_dim<T, 128, sizeof(T) == 4 ? 2 : 4>(a, pl, stream);
+    if (pl.dp == 32) return run_backward_dim<T, 32, 4>(a, pl, sms, stream);
+    if (pl.dp == 64) return run_backward_dim<T, 64, 4>(a, pl, sms, stream);
+    return run_backward_dim<T, 128, sizeof(T) == 4 ? 2 : 4>(a, pl, sms, stream);
 }
 
 template <typename F>

@@ -102,9 +102,15 @@ __device__ __forceinline__ float2 row_stats(float reference, float sum)
 // The forward on the tensor cores of tcgen05 (policy_attention_tc.cu): bf16, tiles of 256 rows.
 constexpr int kTcRows = 256;
 constexpr int kTcKeys = 128;
-// Whether the strides of k and v fit the copies' descriptors: below 2^40 bytes, and keys that are not all
-// the same one.
+// Whether the strides of k and v fit the copies' descriptors (policy_map.h).
 bool attend_tc_takes(const AttnParams& p);
 int launch_attend_tc(const AttnParams& p, int64_t bh, int sms, int device, cudaStream_t stream);
+
+// The gradients on tcgen05 (policy_attention_grad_tc.cu): bf16; dk and dv (keys) or dq.  Takes groups that divide 64
+// and strides that fit the copies' descriptors; p.tiles counts tiles of grad_tc_tile keys or rows.
+bool attend_grad_tc_takes(const AttnParams& p);
+int grad_tc_tile(bool keys, int dim);
+constexpr int kGradTcStream = 64;  // rows or keys that stream past at a time
+int launch_attend_grad_tc(const AttnParams& p, bool keys, int64_t bh, int sms, int device, cudaStream_t stream);
 
 }  // namespace policy

@@ -19,13 +19,12 @@
 // The special function unit gives 16 exponentials a clock and SM: as many clocks for a tile as its products
 // take at dim 128, twice as many at 64.  Replacing a part of them by polynomials on the multiply-add pipes was
 // slower at every share (2 of 8: 2 % at 12,288 x 768 x 128; 4 of 8: 14 %): the issue slots are the scarcer.
-#include <cuda.h>
-
 #include <atomic>
 #include <limits>
 
 #include "policy_attention.cuh"
 #include "policy_internal.h"
+#include "policy_map.h"
 #include "policy_tcgen05.cuh"
 
 namespace policy {
@@ -90,31 +89,6 @@ struct Item {
     __device__ __forceinline__ bool has(const AttnParams& p, int i) const { return r0 + i * kTile < p.rows; }
 };
 
-// two f32 to an instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    float2 r;
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
-        "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}\n"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    float2 r;
-    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 same(float v) { return make_float2(v, v); }
-__device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, int column, int key, int head, int batch, uint32_t bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
-        "l"(map), "r"(column), "r"(key), "r"(head), "r"(batch), "r"(bar)
-        : "memory");
-}
-
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -172,7 +146,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
                 const Item item(p, it);
-                // an axis that the tensor repeats has one entry in the map
                 const int kb = p.ks[0] ? static_cast<int>(item.rows.b) : 0, kh = p.ks[2] ? item.rows.hk : 0;
                 const int vb = p.vs[0] ? static_cast<int>(item.rows.b) : 0, vh = p.vs[2] ? item.rows.hk : 0;
                 for (int t = item.t0; t < item.t1; ++t) {
@@ -181,12 +154,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!(ok = bar_wait(bar(kKEmpty + st), parity, broken))) break;
                     bar_expect(bar(kKFull + st), S::kTileBytes);
                     for (int b = 0; b < S::kBlocks; ++b)
-                        copy_tile(base + S::kK + st * S::kTileBytes + b * S::kBlock, &map_k, b * 64, t * kTile, kh, kb, bar(kKFull + st));
+                        copy_tile(base + S::kK + st * S::kTileBytes + b * S::kBlock, &map_k, b * 64, kh, t * kTile, kb, bar(kKFull + st));
                     ++uses;
                     if (!(ok = bar_wait(bar(kVEmpty + st), parity, broken))) break;
                     bar_expect(bar(kVCopied + st), S::kTileBytes);
                     for (int b = 0; b < S::kBlocks; ++b)
-                        copy_tile(base + S::kV + st * S::kTileBytes + b * S::kBlock, &map_v, b * 64, t * kTile, vh, vb, bar(kVCopied + st));
+                        copy_tile(base + S::kV + st * S::kTileBytes + b * S::kBlock, &map_v, b * 64, vh, t * kTile, vb, bar(kVCopied + st));
                     ++v_uses;
                 }
             }
@@ -558,38 +531,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // --- host ------------------------------------------------------------------------
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled()
-{
-    static const EncodeTiled fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            f = nullptr;
-        }
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return fn;
-}
-
-// Tiles of 64 values x 128 keys of k or v [batch][lk][kv_heads][dim].
-int key_map(CUtensorMap* map, const void* x, const int64_t (&strides)[3], int64_t batch, int lk, int kv_heads, int dim)
-{
-    const EncodeTiled encode = encode_tiled();
-    if (!encode) return fail(POLICY_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    const auto extent = [](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(stride ? n : 1); };
-    const auto bytes = [](int64_t stride) { return static_cast<cuuint64_t>(stride ? stride * 2 : 16); };
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(lk), extent(kv_heads, strides[2]), extent(batch, strides[0])};
-    const cuuint64_t steps[3] = {bytes(strides[1]), bytes(strides[2]), bytes(strides[0])};
-    const cuuint32_t box[4] = {64, kTile, 1, 1}, one[4] = {1, 1, 1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(x), dims, steps, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? POLICY_OK : fail(POLICY_ERR_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string(static_cast<int>(r)));
-}
-
 template <int DP>
 int launch_dim(const AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int items, int sms, int device, cudaStream_t stream)
 {
@@ -606,15 +547,13 @@ int launch_dim(const AttnParams& p, const CUtensorMap& map_k, const CUtensorMap&
     return e == cudaSuccess ? POLICY_OK : cuda_fail(e, "attend_tc_kernel");
 }
 
-bool map_fits(const int64_t (&s)[3], int lk)
-{
-    constexpr int64_t most = (int64_t{1} << 40) / 2;
-    return (s[1] > 0 || lk == 1) && s[0] < most && s[1] < most && s[2] < most && s[0] >= 0 && s[2] >= 0;
-}
-
 }  // namespace
 
-bool attend_tc_takes(const AttnParams& p) { return map_fits(p.ks, p.lk) && map_fits(p.vs, p.lk); }
+bool attend_tc_takes(const AttnParams& p)
+{
+    const int64_t shape[3] = {p.k_count / p.lk / p.kv_heads / p.dim, p.lk, p.kv_heads};
+    return map_takes(shape, p.ks, 1) && map_takes(shape, p.vs, 1);
+}
 
 int launch_attend_tc(const AttnParams& p, int64_t bh, int sms, int device, cudaStream_t stream)
 {
@@ -622,9 +561,10 @@ int launch_attend_tc(const AttnParams& p, int64_t bh, int sms, int device, cudaS
     if (items > std::numeric_limits<int32_t>::max() - 4096)
         return fail(POLICY_ERR_INVALID, "policy_cross_attention: more than 2^31 - 4096 tiles of rows");
     const int64_t batch = bh / p.kv_heads;
+    const int64_t shape[3] = {batch, p.lk, p.kv_heads};
     CUtensorMap map_k, map_v;
-    int rc = key_map(&map_k, p.k, p.ks, batch, p.lk, p.kv_heads, p.dim);
-    if (rc == POLICY_OK) rc = key_map(&map_v, p.v, p.vs, batch, p.lk, p.kv_heads, p.dim);
+    int rc = make_map(&map_k, p.k, shape, p.ks, p.dim, kTile, 1);
+    if (rc == POLICY_OK) rc = make_map(&map_v, p.v, shape, p.vs, p.dim, kTile, 1);
     if (rc != POLICY_OK) return rc;
     return p.dim <= 64 ? launch_dim<64>(p, map_k, map_v, static_cast<int>(items), sms, device, stream)
                        : launch_dim<128>(p, map_k, map_v, static_cast<int>(items), sms, device, stream);
