@@ -124,6 +124,30 @@ __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const
     }
 }
 
+// The products of a 16-row A with N pairs of B tiles, k step by k step: c (+)= a b.  f32 adds up kFlush steps apart
+// and then rounds to nearest, for the same reason.
+constexpr int kFlush = 4;
+
+template <typename T, int STEPS, int N, typename Step>
+__device__ __forceinline__ void multiply(float (&c)[N][4], Step&& step)
+{
+    if constexpr (Mma<T>::kExact) {
+#pragma unroll
+        for (int k0 = 0; k0 < STEPS; k0 += kFlush) {
+            float t[N][4] = {};
+#pragma unroll
+            for (int kk = k0; kk < k0 + kFlush && kk < STEPS; ++kk) step(t, kk);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[j][i] += t[j][i];
+        }
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < STEPS; ++kk) step(c, kk);
+    }
+}
+
 template <typename T, int DP, int WM, int WN, int KT>
 struct FwdShape {
     static constexpr int THREADS = WM * WN * 32;
@@ -206,8 +230,7 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
         for (int j = 0; j < KSL / 8; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < STEPS; ++kk) {
+        multiply<T, STEPS>(s, [&](float (&t)[KSL / 8][4], int kk) {
             typename M::A a;
             if constexpr (QREG) a = qf[kk];
             else M::load_a(a, sq + wm * 16 * PITCH + kk * KS, PITCH, lane);
@@ -215,10 +238,10 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
             for (int j = 0; j < KSL / 16; ++j) {
                 typename M::B b0, b1;
                 M::load_b_nk(b0, b1, tk + j * 16 * PITCH + kk * KS, PITCH, lane);
-                M::mma(s[2 * j], a, b0);
-                M::mma(s[2 * j + 1], a, b1);
+                M::mma(t[2 * j], a, b0);
+                M::mma(t[2 * j + 1], a, b1);
             }
-        }
+        });
         if (p.mask || (t + 1) * KT > n) {
             const uint8_t* vis = svis + st * KT + wn * KSL + (lane & 3) * 2;
 #pragma unroll
@@ -314,27 +337,49 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
     }
 }
 
-// Joins the parts of a forward launch split over the keys: 4 values of a row per thread.
+// Joins the parts of a forward launch split over the keys: a block to a row, its threads in groups of
+// `lanes` (a power of two, 4 values each), which share out the parts.
+constexpr int kJoinThreads = 128;
+
 template <typename T>
-__global__ void __launch_bounds__(128) attend_join_kernel(const AttnParams p)
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttnParams p, int lanes)
 {
-    const int64_t n_rows = p.q_count / p.dim;
-    const int chunks = p.dim / 4;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int64_t row = i / chunks;
-    const int d = static_cast<int>(i - row * chunks) * 4;
-    if (row >= n_rows) return;
+    __shared__ float4 sums[kJoinThreads];
+    __shared__ float2 stats[kJoinThreads];
+    const int64_t n_rows = p.q_count / p.dim, row = blockIdx.x;
+    const int d = (threadIdx.x & (lanes - 1)) * 4, first = threadIdx.x / lanes, groups = kJoinThreads / lanes;
     const float c = p.scale_log2;
-    float m = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (s * n_rows + row)]);
-    const float base = m == -INFINITY ? 0.f : m * c;
-    float l = 0.f;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row;
+    const float* part = p.part + row * p.dim + d;
+    float m = -INFINITY, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (s * n_rows + row));
-        const float f = exp2_fast(fmaf(ml.x, c, -base));
-        const float4 y = *reinterpret_cast<const float4*>(p.part + s * p.q_count + row * p.dim + d);
-        l = fmaf(f, ml.y, l);
+    if (d < p.dim) {
+#pragma unroll 4
+        for (int s = first; s < p.splits; s += groups) {
+            const float2 v = ml[s * n_rows];
+            const float4 y = *reinterpret_cast<const float4*>(part + s * p.q_count);
+            const float top = fmaxf(m, v.x);
+            const float base = top == -INFINITY ? 0.f : top * c;
+            const float a = exp2_fast(fmaf(m, c, -base)), f = exp2_fast(fmaf(v.x, c, -base));
+            m = top;
+            l = fmaf(l, a, f * v.y);
+            x.x = fmaf(x.x, a, f * y.x), x.y = fmaf(x.y, a, f * y.y), x.z = fmaf(x.z, a, f * y.z), x.w = fmaf(x.w, a, f * y.w);
+        }
+    }
+    sums[threadIdx.x] = x;
+    stats[threadIdx.x] = make_float2(m, l);
+    __syncthreads();
+    if (first != 0 || d >= p.dim) return;
+    float top = -INFINITY;
+    for (int g = 0; g < groups; ++g) top = fmaxf(top, stats[g * lanes + threadIdx.x].x);
+    const float base = top == -INFINITY ? 0.f : top * c;
+    l = 0.f;
+    x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = 0; g < groups; ++g) {
+        const float2 v = stats[g * lanes + threadIdx.x];
+        const float4 y = sums[g * lanes + threadIdx.x];
+        const float f = exp2_fast(fmaf(v.x, c, -base));
+        l = fmaf(f, v.y, l);
         x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -489,19 +534,18 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
         T* tk = sk + (st * KT + warp * 16) * PITCH;
         T* tv = sv + (st * KT + warp * 16) * PITCH;
         float s[2][4] = {}, dp[2][4] = {};  // [16 keys] x [16 rows]
-#pragma unroll
-        for (int kk = 0; kk < STEPS; ++kk) {
-            typename M::A ak, av;
-            typename M::B b0, b1;
-            M::load_a(ak, tk + kk * KS, PITCH, lane);
-            M::load_a(av, tv + kk * KS, PITCH, lane);
-            M::load_b_nk(b0, b1, sq + kk * KS, PITCH, lane);
-            M::mma(s[0], ak, b0);
-            M::mma(s[1], ak, b1);
-            M::load_b_nk(b0, b1, sdo + kk * KS, PITCH, lane);
-            M::mma(dp[0], av, b0);
-            M::mma(dp[1], av, b1);
-        }
+        const auto product = [&](float (&out)[2][4], const T* a_tile, const T* b_tile) {
+            multiply<T, STEPS>(out, [&](float (&x)[2][4], int kk) {
+                typename M::A a;
+                typename M::B b0, b1;
+                M::load_a(a, a_tile + kk * KS, PITCH, lane);
+                M::load_b_nk(b0, b1, b_tile + kk * KS, PITCH, lane);
+                M::mma(x[0], a, b0);
+                M::mma(x[1], a, b1);
+            });
+        };
+        product(s, tk, sq);
+        product(dp, tv, sdo);
         const bool on0 = svis[st * KT + warp * 16 + (lane >> 2)], on1 = svis[st * KT + warp * 16 + (lane >> 2) + 8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -650,22 +694,21 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
         const T* tq = sq + st * RT * PITCH;
         const T* td = sdo + st * RT * PITCH;
         float s[RT / 8][4] = {}, dp[RT / 8][4] = {};  // [16 keys] x [RT rows]
+        const auto product = [&](float (&out)[RT / 8][4], const T* a_tile, const T* b_tile) {
+            multiply<T, STEPS>(out, [&](float (&x)[RT / 8][4], int kk) {
+                typename M::A a;
+                M::load_a(a, a_tile + kk * KS, PITCH, lane);
 #pragma unroll
-        for (int kk = 0; kk < STEPS; ++kk) {
-            typename M::A ak, av;
-            M::load_a(ak, tk + kk * KS, PITCH, lane);
-            M::load_a(av, tv + kk * KS, PITCH, lane);
-#pragma unroll
-            for (int j = 0; j < RT / 16; ++j) {
-                typename M::B b0, b1;
-                M::load_b_nk(b0, b1, tq + j * 16 * PITCH + kk * KS, PITCH, lane);
-                M::mma(s[2 * j], ak, b0);
-                M::mma(s[2 * j + 1], ak, b1);
-                M::load_b_nk(b0, b1, td + j * 16 * PITCH + kk * KS, PITCH, lane);
-                M::mma(dp[2 * j], av, b0);
-                M::mma(dp[2 * j + 1], av, b1);
-            }
-        }
+                for (int j = 0; j < RT / 16; ++j) {
+                    typename M::B b0, b1;
+                    M::load_b_nk(b0, b1, b_tile + j * 16 * PITCH + kk * KS, PITCH, lane);
+                    M::mma(x[2 * j], a, b0);
+                    M::mma(x[2 * j + 1], a, b1);
+                }
+            });
+        };
+        product(s, tk, tq);
+        product(dp, tv, td);
 #pragma unroll
         for (int j = 0; j < RT / 8; ++j) {
 #pragma unroll
@@ -793,22 +836,21 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
         const T* tk = sk + st * KT * PITCH;
         const T* tv = sv + st * KT * PITCH;
         float s[KT / 8][4] = {}, dp[KT / 8][4] = {};  // [16 rows] x [KT keys]
+        const auto product = [&](float (&out)[KT / 8][4], const T* a_tile, const T* b_tile) {
+            multiply<T, STEPS>(out, [&](float (&x)[KT / 8][4], int kk) {
+                typename M::A a;
+                M::load_a(a, a_tile + warp * 16 * PITCH + kk * KS, PITCH, lane);
 #pragma unroll
-        for (int kk = 0; kk < STEPS; ++kk) {
-            typename M::A aq, ad;
-            M::load_a(aq, sq + warp * 16 * PITCH + kk * KS, PITCH, lane);
-            M::load_a(ad, sdo + warp * 16 * PITCH + kk * KS, PITCH, lane);
-#pragma unroll
-            for (int j = 0; j < KT / 16; ++j) {
-                typename M::B b0, b1;
-                M::load_b_nk(b0, b1, tk + j * 16 * PITCH + kk * KS, PITCH, lane);
-                M::mma(s[2 * j], aq, b0);
-                M::mma(s[2 * j + 1], aq, b1);
-                M::load_b_nk(b0, b1, tv + j * 16 * PITCH + kk * KS, PITCH, lane);
-                M::mma(dp[2 * j], ad, b0);
-                M::mma(dp[2 * j + 1], ad, b1);
-            }
-        }
+                for (int j = 0; j < KT / 16; ++j) {
+                    typename M::B b0, b1;
+                    M::load_b_nk(b0, b1, b_tile + j * 16 * PITCH + kk * KS, PITCH, lane);
+                    M::mma(x[2 * j], a, b0);
+                    M::mma(x[2 * j + 1], a, b1);
+                }
+            });
+        };
+        product(s, sq, tk);
+        product(dp, sdo, tv);
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
             const uchar2 vis = *reinterpret_cast<const uchar2*>(svis + st * KT + j * 8 + (lane & 3) * 2);
@@ -975,13 +1017,27 @@ struct Plan {
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-// Blocks to aim at, as blocks per SM that a launch of this kind keeps resident; a split below two
-// tiles would cost more in parts than it gives.
-int choose_splits(int64_t blocks, int tiles, int sms, int per_sm = 4)
+// How many parts a long axis of `tiles` tiles is split into when there are `blocks` blocks: as many as keep one
+// full set of resident blocks, none shorter than `least` tiles (a shorter one costs more in parts than it gives).
+int choose_splits(int64_t blocks, int tiles, int64_t resident, int least)
 {
-    const int64_t want = (static_cast<int64_t>(sms) * per_sm + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = tiles / 2 > 1 ? tiles / 2 : 1;
-    return static_cast<int>(want < 1 ? 1 : want < most ? want : most);
+    const int64_t want = resident / (blocks > 0 ? blocks : 1);
+    const int64_t most = tiles / least;
+    const int64_t n = want < most ? want : most;
+    return static_cast<int>(n > 1 ? n : 1);
+}
+
+// Blocks of `bytes` of shared memory that are resident on the device, at most `most` an SM (their registers).
+int64_t resident_blocks(size_t bytes, int most, int sms)
+{
+    const int n = static_cast<int>((228 * 1024) / (bytes + 1024));
+    return static_cast<int64_t>(sms) * (n < 1 ? 1 : n < most ? n : most);
+}
+
+size_t fwd_bytes(bool f32, int dp, int rows, int keys)
+{
+    const size_t pitch = f32 ? 4 * (dp + 4) : 2 * (dp + 8);
+    return pitch * (rows + 4 * keys);
 }
 
 // From this many rows on the gradients run on tcgen05.
@@ -996,29 +1052,31 @@ Plan make_plan(const policy_attention& a, int sms)
     pl.dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
     pl.fwd_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     if (f32) pl.fwd_keys = pl.dp == 128 ? 32 : 64;
-    else pl.fwd_keys = pl.dp == 128 || pl.fwd_rows == 64 ? 64 : 128;
+    else pl.fwd_keys = 64;
     pl.tc = !f32 && rows > 64 && attend_tc_takes(make_params(a));
     if (pl.tc) pl.fwd_rows = kTcRows, pl.fwd_keys = kTcKeys;
     pl.grad_warps = f32 && pl.dp == 128 ? 2 : 4;
     const int64_t q_count = a.batch * a.lq * a.heads * a.dim, k_count = a.batch * a.lk * a.kv_heads * a.dim;
     if (bh == 0) return pl;
-    pl.fwd_splits = choose_splits(bh * ceil_div(rows, pl.fwd_rows), ceil_div(a.lk, pl.fwd_keys), sms, pl.tc ? 1 : 4);
+    const int64_t fwd_resident = pl.tc ? sms : resident_blocks(fwd_bytes(f32, pl.dp, pl.fwd_rows, pl.fwd_keys), 5, sms);
+    pl.fwd_splits = choose_splits(bh * ceil_div(rows, pl.fwd_rows), ceil_div(a.lk, pl.fwd_keys), fwd_resident, pl.tc ? 2 : 4);
     if (pl.fwd_splits > 1)
         pl.fwd_bytes = align256(sizeof(float) * pl.fwd_splits * q_count) + align256(sizeof(float) * 2 * pl.fwd_splits * (q_count / a.dim));
     pl.few = rows <= 16;
     const int kt = pl.grad_warps * 16;
     if (pl.few) {
-        pl.few_splits = choose_splits(bh, ceil_div(a.lk, kt), sms);
+        pl.few_splits = choose_splits(bh, ceil_div(a.lk, kt), resident_blocks(fwd_bytes(f32, pl.dp, 32, kt), 4, sms), 4);
         if (pl.few_splits > 1) pl.grad_bytes = align256(sizeof(float) * pl.few_splits * q_count);
     } else {
         pl.grad_bytes = align256(sizeof(float) * (q_count / a.dim));
         pl.grad_tc = !f32 && rows > kTcGradRows && attend_grad_tc_takes(make_params(a));
         if (pl.grad_tc) {
-            pl.key_splits = choose_splits(bh * ceil_div(a.lk, grad_tc_tile(true, a.dim)), ceil_div(rows, kGradTcStream), sms, 2);
-            pl.query_splits = choose_splits(bh * ceil_div(rows, grad_tc_tile(false, a.dim)), ceil_div(a.lk, kGradTcStream), sms, 1);
+            // items differ in length where lengths do: two for each SM
+            pl.key_splits = choose_splits(bh * ceil_div(a.lk, grad_tc_tile(true, a.dim)), ceil_div(rows, kGradTcStream), 2 * sms, 4);
+            pl.query_splits = choose_splits(bh * ceil_div(rows, grad_tc_tile(false, a.dim)), ceil_div(a.lk, kGradTcStream), sms, 4);
         } else {
-            pl.key_splits = choose_splits(bh * ceil_div(a.lk, kt), ceil_div(rows, 32), sms);
-            pl.query_splits = choose_splits(bh * ceil_div(rows, kt), ceil_div(a.lk, 32), sms);
+            pl.key_splits = choose_splits(bh * ceil_div(a.lk, kt), ceil_div(rows, 32), 4 * sms, 2);
+            pl.query_splits = choose_splits(bh * ceil_div(rows, kt), ceil_div(a.lk, 32), 4 * sms, 4);
         }
         if (pl.key_splits > 1) pl.grad_bytes += align256(sizeof(float) * 2 * pl.key_splits * k_count);
         if (pl.query_splits > 1) pl.grad_bytes += align256(sizeof(float) * pl.query_splits * q_count);
@@ -1074,7 +1132,7 @@ int launch_fwd_rows(const AttnParams& p, const Plan& pl, int64_t bh, int device,
         if (pl.fwd_rows == 32) return launch_fwd<T, DP, 2, 1, 32>(p, bh, device, stream);
         return launch_fwd<T, DP, 4, 1, 32>(p, bh, device, stream);
     } else {
-        constexpr int KN = f32 || DP == 128 ? 64 : 128;
+        constexpr int KN = 64;
         if (pl.fwd_rows == 16) return launch_fwd<T, DP, 1, 4, KN>(p, bh, device, stream);
         if (pl.fwd_rows == 32) return launch_fwd<T, DP, 2, 2, KN>(p, bh, device, stream);
         return launch_fwd<T, DP, 4, 1, 64>(p, bh, device, stream);
@@ -1098,8 +1156,10 @@ int run_forward(const policy_attention& a, const Plan& pl, int sms, cudaStream_t
                            : launch_fwd_rows<T, 128>(p, pl, bh, a.device, stream);
     if (rc != POLICY_OK || p.splits == 1) return rc;
     unsigned grid = 0;
-    if ((rc = launch_blocks((p.q_count / 4 + 127) / 128, "policy_cross_attention", grid)) != POLICY_OK) return rc;
-    attend_join_kernel<T><<<grid, 128, 0, stream>>>(p);
+    if ((rc = launch_blocks(p.q_count / p.dim, "policy_cross_attention", grid)) != POLICY_OK) return rc;
+    int lanes = 2;
+    while (lanes * 4 < p.dim) lanes *= 2;
+    attend_join_kernel<T><<<grid, kJoinThreads, 0, stream>>>(p, lanes);
     return launched("attend_join_kernel");
 }
 

@@ -17,7 +17,7 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;        // values: 16 per thread
+constexpr int kChunk = 8192;        // values: 32 per thread, all in flight at once
 constexpr int kBlocksPerSm = 8;     // 256 threads: the SM is full
 constexpr int kMaxSms = 256;         // SMs that the workspace allows for
 constexpr int kTensors = 512;       // tensors of one launch (its parameters: 16 KB)
@@ -96,11 +96,11 @@ __global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_consta
         if (n == kChunk && (t.dtype & 2u)) {
             if (t.dtype & 1u) {
                 const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.grad) + at);
-                uint4 v[2];
+                uint4 v[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) v[i] = g[threadIdx.x + i * kThreads];
+                for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -110,11 +110,11 @@ __global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_consta
                 }
             } else {
                 const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
-                float4 v[4];
+                float4 v[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
+                for (int i = 0; i < 8; ++i) v[i] = g[threadIdx.x + i * kThreads];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 8; ++i)
                     x = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, fmaf(v[i].z, v[i].z, fmaf(v[i].w, v[i].w, x))));
             }
         } else {
@@ -149,20 +149,20 @@ __global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_const
             if (t.dtype & 1u) {
                 const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.grad) + at);
                 uint4* o = reinterpret_cast<uint4*>(static_cast<bf16*>(t.out) + at);
-                uint4 v[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) v[i] = g[threadIdx.x + i * kThreads];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    o[threadIdx.x + i * kThreads] = make_uint4(scale2(v[i].x, c), scale2(v[i].y, c), scale2(v[i].z, c), scale2(v[i].w, c));
-            } else {
-                const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
-                float4* o = reinterpret_cast<float4*>(static_cast<float*>(t.out) + at);
-                float4 v[4];
+                uint4 v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
+                    o[threadIdx.x + i * kThreads] = make_uint4(scale2(v[i].x, c), scale2(v[i].y, c), scale2(v[i].z, c), scale2(v[i].w, c));
+            } else {
+                const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
+                float4* o = reinterpret_cast<float4*>(static_cast<float*>(t.out) + at);
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = g[threadIdx.x + i * kThreads];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
                     o[threadIdx.x + i * kThreads] = make_float4(v[i].x * c, v[i].y * c, v[i].z * c, v[i].w * c);
             }
         } else {

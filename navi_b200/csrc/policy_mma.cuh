@@ -106,13 +106,13 @@ struct Mma<float> {
     struct A { float r[4]; };
     struct B { float r[2]; };
 
+    // hi: the value rounded to TF32's 11 bits (half away from zero), by integers: the conversion instruction runs at
+    // a fraction of their rate.  lo: what is left, of which the tensor core drops all below 2^-22 of the value.  An
+    // infinite value leaves inf - inf and so gives NaN.
     static __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo)
     {
-        asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(hi) : "f"(x));
-        // rounded, not left to the tensor core to truncate: that would be a bias of 2^-22 of every product
-        asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
-        // an infinite value leaves inf - inf here: its products are already infinite through hi
-        if ((hi & 0x7f800000u) == 0x7f800000u) lo = 0u;
+        hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+        lo = __float_as_uint(x - __uint_as_float(hi));
     }
     static __device__ __forceinline__ void mma1(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2])
     {

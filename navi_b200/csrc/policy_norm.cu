@@ -198,9 +198,13 @@ __device__ __forceinline__ void load_weight(F2 (&w)[4], const NormSide& s, int s
     }
 }
 
+// Rows that a thread works on at a time: HEADS heads of its token in kRows / HEADS batches.
+constexpr int kRows = 4;
+
 template <typename T, int LANES, int HEADS>
 __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant__ NormParams p)
 {
+    constexpr int BATCHES = kRows / HEADS;
     const bool second = blockIdx.x >= p.side[0].blocks;
     const NormSide& s = p.side[second ? 1 : 0];
     const Work<LANES, HEADS> at(p, s, second ? blockIdx.x - p.side[0].blocks : blockIdx.x);
@@ -209,55 +213,65 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant
     bool inside = true;
     if (s.table && !s.positions) inside = angles(p, s, at, at.token, cs, sn);
 
-    const int rounds = __reduce_max_sync(0xffffffffu, at.b1 - at.b0);
+    const int rounds = __reduce_max_sync(0xffffffffu, (at.b1 - at.b0 + BATCHES - 1) / BATCHES);
     const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
-    T* y = static_cast<T*>(s.y) + ((static_cast<int64_t>(at.b0) * s.tokens + at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
     const int64_t y_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
-    Raw<T> next[HEADS];
-    int64_t next_pos = 0;
-    auto fetch = [&](int i) {
-        const bool on = at.b0 + i < at.b1;
+    T* y = static_cast<T*>(s.y) + at.b0 * y_step + (static_cast<int64_t>(at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
+    Raw<T> next[kRows];
+    int next_pos[BATCHES] = {};
+    const auto here = [&](int i, int u) { return at.b0 + i * BATCHES + u < at.b1; };
+    const auto fetch = [&](int i) {
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            if (on && h < at.heads) next[h].load(x + i * s.xs[0] + h * s.xs[2]);
-            else next[h].clear();
+        for (int u = 0; u < BATCHES; ++u) {
+            const int64_t b = i * BATCHES + u;
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) {
+                if (here(i, u) && h < at.heads) next[u * HEADS + h].load(x + b * s.xs[0] + h * s.xs[2]);
+                else next[u * HEADS + h].clear();
+            }
+            if (s.positions && here(i, u)) next_pos[u] = s.positions[(at.b0 + b) * s.tokens + at.token];
         }
-        if (s.positions && on) next_pos = s.positions[static_cast<int64_t>(at.b0 + i) * s.tokens + at.token];
     };
     fetch(0);
     for (int i = 0; i < rounds; ++i) {
-        F2 v[HEADS][4];
+        F2 v[kRows][4];
+        int pos[BATCHES];
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) next[h].get(v[h]);
-        const int64_t pos = next_pos;
+        for (int k = 0; k < kRows; ++k) next[k].get(v[k]);
+#pragma unroll
+        for (int u = 0; u < BATCHES; ++u) pos[u] = next_pos[u];
         if (i + 1 < rounds) fetch(i + 1);
-        if (s.positions) inside = angles(p, s, at, pos, cs, sn);
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            F2 sum = mul2(v[h][0], v[h][0]);
+        for (int u = 0; u < BATCHES; ++u) {
+            if (s.positions) inside = angles(p, s, at, pos[u], cs, sn);
 #pragma unroll
-            for (int k = 1; k < 4; ++k) sum = fma2(v[h][k], v[h][k], sum);
-            const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
-            const F2 r2 = pair(r, r);
+            for (int h = 0; h < HEADS; ++h) {
+                F2(&z)[4] = v[u * HEADS + h];
+                F2 sum = mul2(z[0], z[0]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[h][k] = mul2(mul2(v[h][k], r2), w[k]);
-            if (s.table) {
+                for (int k = 1; k < 4; ++k) sum = fma2(z[k], z[k], sum);
+                const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
+                const F2 r2 = pair(r, r);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const F2 o = shuffle2(v[h][k], at.other);
-                    v[h][k] = fma2(v[h][k], cs[k], mul2(o, sn[k]));
-                    if (!inside) v[h][k] = pair(NAN, NAN);
+                for (int k = 0; k < 4; ++k) z[k] = mul2(mul2(z[k], r2), w[k]);
+                if (s.table) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const F2 o = shuffle2(z[k], at.other);
+                        z[k] = fma2(z[k], cs[k], mul2(o, sn[k]));
+                        if (!inside) z[k] = pair(NAN, NAN);
+                    }
                 }
+                if (h < at.heads && here(i, u)) Raw<T>::store(y + (i * BATCHES + u) * y_step + h * p.dim, z);
             }
-            if (h < at.heads && at.b0 + i < at.b1) Raw<T>::store(y + h * p.dim, v[h]);
         }
-        y += y_step;
     }
 }
 
 template <typename T, int LANES, int HEADS>
 __global__ void __launch_bounds__(kThreads) qk_norm_grad_kernel(const __grid_constant__ NormParams p)
 {
+    constexpr int BATCHES = kRows / HEADS;
     __shared__ float sums[kThreads * 8];
     const bool second = blockIdx.x >= p.side[0].blocks;
     const NormSide& s = p.side[second ? 1 : 0];
@@ -270,64 +284,71 @@ __global__ void __launch_bounds__(kThreads) qk_norm_grad_kernel(const __grid_con
     bool inside = true;
     if (s.table && !s.positions) inside = angles(p, s, at, at.token, cs, sn);
 
-    const int rounds = __reduce_max_sync(0xffffffffu, at.b1 - at.b0);
+    const int rounds = __reduce_max_sync(0xffffffffu, (at.b1 - at.b0 + BATCHES - 1) / BATCHES);
     const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
     const T* dy = static_cast<const T*>(s.dy) + at.b0 * s.ds[0] + at.token * s.ds[1] + at.h0 * s.ds[2] + at.sub * 8;
-    T* dx = static_cast<T*>(s.y) + ((static_cast<int64_t>(at.b0) * s.tokens + at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
     const int64_t dx_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
+    T* dx = static_cast<T*>(s.y) + at.b0 * dx_step + (static_cast<int64_t>(at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
     for (int i = 0; i < rounds; ++i) {
-        const bool on = at.b0 + i < at.b1;
-        Raw<T> rx[HEADS], rg[HEADS];
+        Raw<T> rx[kRows], rg[kRows];
+        int pos[BATCHES];
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            if (on && h < at.heads) {
-                rx[h].load(x + i * s.xs[0] + h * s.xs[2]);
-                rg[h].load(dy + i * s.ds[0] + h * s.ds[2]);
-            } else {
-                rx[h].clear();
-                rg[h].clear();
-            }
-        }
-        if (s.positions) {
-            int64_t pos = at.token;
-            if (on) pos = s.positions[static_cast<int64_t>(at.b0 + i) * s.tokens + at.token];
-            inside = angles(p, s, at, pos, cs, sn);
-        }
+        for (int u = 0; u < BATCHES; ++u) {
+            const int64_t b = i * BATCHES + u;
+            const bool on = at.b0 + b < at.b1;
+            pos[u] = at.token;
+            if (s.positions && on) pos[u] = s.positions[(at.b0 + b) * s.tokens + at.token];
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            const bool here = on && h < at.heads;
-            F2 v[4], g[4];
-            rx[h].get(v);
-            rg[h].get(g);
-            if (s.table) {  // the rotation back: the sines change sign
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const F2 o = shuffle2(g[k], at.other);
-                    g[k] = fma2(g[k], cs[k], mul2(mul2(o, sn[k]), pair(-1.f, -1.f)));
-                    if (!inside && here) g[k] = pair(NAN, NAN);
+            for (int h = 0; h < HEADS; ++h) {
+                const int k = u * HEADS + h;
+                if (on && h < at.heads) {
+                    rx[k].load(x + b * s.xs[0] + h * s.xs[2]);
+                    rg[k].load(dy + b * s.ds[0] + h * s.ds[2]);
+                } else {
+                    rx[k].clear();
+                    rg[k].clear();
                 }
             }
-            F2 sum = mul2(v[0], v[0]), dot = mul2(mul2(v[0], w[0]), g[0]);
+        }
 #pragma unroll
-            for (int k = 1; k < 4; ++k) {
-                sum = fma2(v[k], v[k], sum);
-                dot = fma2(mul2(v[k], w[k]), g[k], dot);
-            }
-            const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
-            const float f = -r * r * r * (row_sum<LANES>(dot) * p.inv_dim);
-            const F2 r2 = pair(r, r), f2 = pair(f, f);
-            if (here) {
-                F2 d[4];
+        for (int u = 0; u < BATCHES; ++u) {
+            const int64_t b = i * BATCHES + u;
+            if (s.positions) inside = angles(p, s, at, pos[u], cs, sn);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const F2 gr = mul2(g[k], r2);
-                    dw[k] = fma2(gr, v[k], dw[k]);
-                    d[k] = fma2(gr, w[k], mul2(f2, v[k]));
+            for (int h = 0; h < HEADS; ++h) {
+                const bool here = at.b0 + b < at.b1 && h < at.heads;
+                F2 v[4], g[4];
+                rx[u * HEADS + h].get(v);
+                rg[u * HEADS + h].get(g);
+                if (s.table) {  // the rotation back: the sines change sign
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const F2 o = shuffle2(g[k], at.other);
+                        g[k] = fma2(g[k], cs[k], mul2(mul2(o, sn[k]), pair(-1.f, -1.f)));
+                        if (!inside && here) g[k] = pair(NAN, NAN);
+                    }
                 }
-                Raw<T>::store(dx + h * p.dim, d);
+                F2 sum = mul2(v[0], v[0]), dot = mul2(mul2(v[0], w[0]), g[0]);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) {
+                    sum = fma2(v[k], v[k], sum);
+                    dot = fma2(mul2(v[k], w[k]), g[k], dot);
+                }
+                const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
+                const float f = -r * r * r * (row_sum<LANES>(dot) * p.inv_dim);
+                const F2 r2 = pair(r, r), f2 = pair(f, f);
+                if (here) {
+                    F2 d[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const F2 gr = mul2(g[k], r2);
+                        dw[k] = fma2(gr, v[k], dw[k]);
+                        d[k] = fma2(gr, w[k], mul2(f2, v[k]));
+                    }
+                    Raw<T>::store(dx + b * dx_step + h * p.dim, d);
+                }
             }
         }
-        dx += dx_step;
     }
     if (!s.part) return;
     // the block's rows, in order
@@ -345,23 +366,24 @@ __global__ void __launch_bounds__(kThreads) qk_norm_grad_kernel(const __grid_con
     }
 }
 
-// dweight[d] = sum of the blocks' parts: one block per (side, 32 columns), 32 threads to a column.
+// dweight[d] = sum of the blocks' parts: a block to 8 columns (one 32-byte sector) of a side, 128 threads to a
+// column, so that the few thousand parts are a few dependent reads.
 __global__ void __launch_bounds__(1024) norm_weight_kernel(const __grid_constant__ NormParams p)
 {
-    __shared__ float sums[32][33];
+    __shared__ float sums[128][9];
     const NormSide& s = p.side[blockIdx.y];
     if (!s.part) return;
-    const int d = blockIdx.x * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
+    const int column = threadIdx.x & 7, first = threadIdx.x >> 3, d = blockIdx.x * 8 + column;
     float x = 0.f;
-    if (d < p.dim)
-        for (int r = r0; r < s.blocks; r += 32) x += s.part[static_cast<int64_t>(r) * p.dim + d];
-    sums[r0][threadIdx.x & 31] = x;
+#pragma unroll 4
+    for (int r = first; r < s.blocks; r += 128) x += s.part[static_cast<int64_t>(r) * p.dim + d];
+    sums[first][column] = x;
     __syncthreads();
-    if (r0 == 0 && d < p.dim) {
-        x = 0.f;
-        for (int r = 0; r < 32; ++r) x += sums[r][threadIdx.x];
-        s.dweight[d] = x;
+    for (int n = 64; n > 0; n >>= 1) {
+        if (first < n) sums[first][column] += sums[first + n][column];
+        __syncthreads();
     }
+    if (first == 0) s.dweight[d] = sums[0][column];
 }
 
 // --- host ----------------------------------------------------------------------
@@ -452,7 +474,8 @@ int make_norm(const policy_qk_norm& a, int sms, bool backward, NormParams& p)
         total += a.batch * s.tokens * d.chunks;
     }
     const int64_t want = static_cast<int64_t>(sms) * kBlocksPerSm * kRounds * groups;
-    const int64_t length = total / want > 1 ? total / want : 1;  // batches of a thread
+    const int64_t round = kRows / shape.heads;  // batches at a time
+    const int64_t length = total / want > 1 ? (total / want + round - 1) / round * round : 1;  // batches of a thread
     for (NormSide& d : p.side) {
         d.splits = static_cast<int>((a.batch + length - 1) / length);
         const int64_t blocks = (static_cast<int64_t>(d.splits) * d.tokens * d.chunks + groups - 1) / groups;
@@ -520,7 +543,7 @@ int run_norm(const policy_qk_norm* a, bool backward, cudaStream_t stream)
         if (e != cudaSuccess) return cuda_fail(e, "qk_norm_kernel");
     }
     if (weights) {
-        norm_weight_kernel<<<dim3((p.dim + 31) / 32, 2), 1024, 0, stream>>>(p);
+        norm_weight_kernel<<<dim3(p.dim / 8, 2), 1024, 0, stream>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "norm_weight_kernel");
     }

@@ -11,7 +11,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <unordered_set>
 #include <vector>
 
 #include "policy.h"
@@ -348,8 +347,8 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
     const at::Device device = grads[0].device();
     REQUIRE(device.is_cuda(), "grads must be CUDA tensors. CPU tensors are not supported.");
     std::vector<policy_grad> table(grads.size());
-    std::unordered_set<const void*> written;
-    written.reserve(2 * grads.size());
+    std::vector<const void*> written;
+    written.reserve(grads.size());
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor &g = grads[i], &o = outs[i];
         REQUIRE(known_type(g), "grads must be float32 or bfloat16");
@@ -361,8 +360,10 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
         table[i].out = o.data_ptr();
         table[i].count = static_cast<uint64_t>(g.numel());
         table[i].dtype = dtype_of(g);
-        REQUIRE(g.numel() == 0 || written.insert(table[i].out).second, "the tensors that are written must not share memory");
+        if (table[i].count) written.push_back(table[i].out);
     }
+    std::sort(written.begin(), written.end());
+    REQUIRE(std::adjacent_find(written.begin(), written.end()) == written.end(), "the tensors that are written must not share memory");
     at::NoGradGuard no_grad;
     const auto n = static_cast<int64_t>(table.size());
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
