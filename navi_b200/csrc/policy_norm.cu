@@ -11,17 +11,16 @@
 // are worked on.  Everything between the read and the one rounding at the store is in 32 bits, two
 // values to an instruction (the f32x2 forms), since at 16 bits a value the issue slots come next
 // after memory.
-#include <cuda_bf16.h>
-
+#include <atomic>
 #include <cmath>
 #include <limits>
 
 #include "policy_internal.h"
+#include "policy_mma.cuh"
 
 namespace policy {
 namespace {
 
-using bf16 = __nv_bfloat16;
 constexpr int kThreads = 256;
 
 struct NormSide {
@@ -84,12 +83,31 @@ template <typename T>
 struct Raw;
 template <>
 struct Raw<float> {
+    static constexpr int kPieces = 2;  // of 16 bytes
+    // by way of L1: the two halves of a sector are two copies
+    static __device__ __forceinline__ void copy(uint32_t dst, const float* src, bool take)
+    {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+    }
     float4 a, b;
+    __device__ __forceinline__ void fill(float v) { a = b = make_float4(v, v, v, v); }
+    __device__ __forceinline__ void take(const uint4* ring)
+    {
+        a = *reinterpret_cast<const float4*>(ring), b = *reinterpret_cast<const float4*>(ring + kThreads);
+    }
     __device__ __forceinline__ void load(const float* p)
     {
         a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
     }
-    __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ Raw from(int lane) const
+    {
+        Raw r;
+        r.a.x = __shfl_sync(0xffffffffu, a.x, lane), r.a.y = __shfl_sync(0xffffffffu, a.y, lane);
+        r.a.z = __shfl_sync(0xffffffffu, a.z, lane), r.a.w = __shfl_sync(0xffffffffu, a.w, lane);
+        r.b.x = __shfl_sync(0xffffffffu, b.x, lane), r.b.y = __shfl_sync(0xffffffffu, b.y, lane);
+        r.b.z = __shfl_sync(0xffffffffu, b.z, lane), r.b.w = __shfl_sync(0xffffffffu, b.w, lane);
+        return r;
+    }
     __device__ __forceinline__ void get(F2 (&v)[4]) const
     {
         v[0] = pair(a.x, a.y), v[1] = pair(a.z, a.w), v[2] = pair(b.x, b.y), v[3] = pair(b.z, b.w);
@@ -103,9 +121,18 @@ struct Raw<float> {
 };
 template <>
 struct Raw<bf16> {
+    static constexpr int kPieces = 1;
+    static __device__ __forceinline__ void copy(uint32_t dst, const bf16* src, bool take) { copy16(dst, src, take); }
     uint4 a;
-    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void clear() { a = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void take(const uint4* ring) { a = *ring; }
+    // the values of another lane, two to a shuffle
+    __device__ __forceinline__ Raw from(int lane) const
+    {
+        Raw r;
+        r.a.x = __shfl_sync(0xffffffffu, a.x, lane), r.a.y = __shfl_sync(0xffffffffu, a.y, lane);
+        r.a.z = __shfl_sync(0xffffffffu, a.z, lane), r.a.w = __shfl_sync(0xffffffffu, a.w, lane);
+        return r;
+    }
     static __device__ __forceinline__ F2 one(uint32_t w)
     {
         return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -163,29 +190,60 @@ struct Work {
     }
 };
 
-// The cosines and signed sines of a lane's 8 values, y = u cos + other sin; false for a position
-// outside the table.
-template <int LANES, int HEADS>
-__device__ __forceinline__ bool angles(const NormParams& p, const NormSide& s, const Work<LANES, HEADS>& at, int64_t pos, F2 (&cs)[4],
-                                       F2 (&sn)[4])
-{
-    const bool inside = pos >= 0 && pos < s.table_rows;
-    if (at.active && inside && at.turned) {
-        const float* row = s.table + pos * p.rotary + (at.low ? at.sub : at.sub - p.rotary / 16) * 8;
-        Raw<float> c, n;
-        c.load(row);
-        n.load(row + p.rotary / 2);
+// The cosines and sines of a lane's 8 values, y = u cos + other sin: the sine is negative in the first half of a
+// pair (backward: in the second).  Outside the table both are NaN, and so is every value that they meet.
+struct Angles {
+    Raw<float> c, n;
+    template <int LANES, int HEADS>
+    __device__ __forceinline__ void load(const NormParams& p, const NormSide& s, const Work<LANES, HEADS>& at, int pos)
+    {
+        const bool inside = pos >= 0 && pos < s.table_rows;
+        if (at.active && inside && at.turned) {
+            const float* row = s.table + static_cast<int64_t>(pos) * p.rotary + (at.low ? at.sub : at.sub - p.rotary / 16) * 8;
+            c.load(row);
+            n.load(row + p.rotary / 2);
+        } else {
+            c.fill(inside || !at.active ? 1.f : NAN);
+            n.fill(0.f);
+        }
+    }
+    __device__ __forceinline__ void get(bool negative, F2 (&cs)[4], F2 (&sn)[4]) const
+    {
         c.get(cs);
         n.get(sn);
-        const float sign = at.low ? -1.f : 1.f;
+        const float sign = negative ? -1.f : 1.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sn[i] = mul2(sn[i], pair(sign, sign));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cs[i] = pair(1.f, 1.f), sn[i] = pair(0.f, 0.f);
     }
-    return inside;
-}
+};
+
+// The positions of a thread's token, batch by batch: the angles of the next round are read while this round's rows
+// are worked on, the position after it at the same time.
+template <int LANES, int HEADS>
+struct Positions {
+    const NormParams& p;
+    const NormSide& s;
+    const Work<LANES, HEADS>& at;
+    Angles now;
+    int following;
+    __device__ __forceinline__ int position(int i) const
+    {
+        const int64_t b = at.b0 + i;
+        return !s.positions ? at.token : b < at.b1 ? s.positions[b * s.tokens + at.token] : 0;
+    }
+    __device__ __forceinline__ Positions(const NormParams& p_, const NormSide& s_, const Work<LANES, HEADS>& at_) : p(p_), s(s_), at(at_)
+    {
+        now.load(p, s, at, position(0));
+        following = position(1);
+    }
+    __device__ __forceinline__ Angles next(int i)
+    {
+        const Angles current = now;
+        now.load(p, s, at, following);
+        following = position(i + 2);
+        return current;
+    }
+};
 
 __device__ __forceinline__ void load_weight(F2 (&w)[4], const NormSide& s, int sub, bool active)
 {
@@ -198,160 +256,223 @@ __device__ __forceinline__ void load_weight(F2 (&w)[4], const NormSide& s, int s
     }
 }
 
-// Rows that a thread works on at a time: HEADS heads of its token in kRows / HEADS batches.
-constexpr int kRows = 4;
+// Rows that a thread works on at a time: HEADS heads of its token, in as many batches as make kRows of them (one with
+// positions, where each batch has its own angles).
+template <typename T>
+constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
 
-template <typename T, int LANES, int HEADS>
-__global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant__ NormParams p)
+// The rows of the next rounds come by asynchronous copies into the thread's own places of a ring in shared memory
+// (no other thread reads them, so no barrier): with the rows in registers instead, too few bytes were on their way
+// (16 warps an SM, 4.5 TB/s).  TENSORS: x, or x and dy.
+template <typename T, int HEADS, int TENSORS, bool POSITIONS>
+struct Ring {
+    static constexpr int BATCHES = POSITIONS ? 1 : kRows<T> / HEADS;
+    static constexpr int ROWS = BATCHES * HEADS;
+    static constexpr int kPieces = TENSORS * ROWS * Raw<T>::kPieces;  // 16-byte places of a stage
+    static constexpr int kStages = kPieces <= 4 ? 4 : sizeof(T) == 4 ? 2 : 3;
+    static constexpr size_t kBytes = sizeof(uint4) * kStages * kPieces * kThreads;
+
+    uint4* mine;
+    const T* x[TENSORS];
+    int64_t batch[TENSORS], head[TENSORS];  // strides
+    int b0, b1, heads;
+
+    __device__ __forceinline__ void issue(int i)
+    {
+        uint4* to = mine + (i % kStages) * kPieces * kThreads;
+#pragma unroll
+        for (int t = 0; t < TENSORS; ++t) {
+#pragma unroll
+            for (int u = 0; u < BATCHES; ++u) {
+                const int64_t b = static_cast<int64_t>(i) * BATCHES + u;
+                const bool on = b0 + b < b1;
+#pragma unroll
+                for (int h = 0; h < HEADS; ++h) {
+                    const bool take = on && h < heads;
+                    const T* from = take ? x[t] + b * batch[t] + h * head[t] : x[t];
+#pragma unroll
+                    for (int c = 0; c < Raw<T>::kPieces; ++c, to += kThreads) Raw<T>::copy(smem_addr(to), from + c * (16 / sizeof(T)), take);
+                }
+            }
+        }
+        copy_commit();
+    }
+    __device__ __forceinline__ void start()
+    {
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) issue(i);
+    }
+    // the rows of round i are there, and the round kStages - 1 later is on its way
+    __device__ __forceinline__ const uint4* round(int i)
+    {
+        copy_wait<kStages - 2>();
+        return mine + (i % kStages) * kPieces * kThreads;
+    }
+};
+
+template <typename T, int LANES, int HEADS, bool POSITIONS>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !POSITIONS ? 3 : 2) qk_norm_kernel(const __grid_constant__ NormParams p)
 {
-    constexpr int BATCHES = kRows / HEADS;
+    using R = Ring<T, HEADS, 1, POSITIONS>;
+    extern __shared__ uint4 ring_memory[];
     const bool second = blockIdx.x >= p.side[0].blocks;
     const NormSide& s = p.side[second ? 1 : 0];
     const Work<LANES, HEADS> at(p, s, second ? blockIdx.x - p.side[0].blocks : blockIdx.x);
-    F2 w[4], cs[4], sn[4];
-    load_weight(w, s, at.sub, at.active);
-    bool inside = true;
-    if (s.table && !s.positions) inside = angles(p, s, at, at.token, cs, sn);
-
-    const int rounds = __reduce_max_sync(0xffffffffu, (at.b1 - at.b0 + BATCHES - 1) / BATCHES);
+    const int rounds = __reduce_max_sync(0xffffffffu, (at.b1 - at.b0 + R::BATCHES - 1) / R::BATCHES);
     const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
+    R ring{ring_memory + threadIdx.x, {x}, {s.xs[0]}, {s.xs[2]}, at.b0, at.b1, at.heads};
+    ring.start();
     const int64_t y_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
     T* y = static_cast<T*>(s.y) + at.b0 * y_step + (static_cast<int64_t>(at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
-    Raw<T> next[kRows];
-    int next_pos[BATCHES] = {};
-    const auto here = [&](int i, int u) { return at.b0 + i * BATCHES + u < at.b1; };
-    const auto fetch = [&](int i) {
+
+    // y = r (x (w cos) + other x (other w sin)): the products with the weights are made once for all rows of a token
+    F2 w[4], wo[4], cs[4], sn[4];
+    load_weight(w, s, at.sub, at.active);
 #pragma unroll
-        for (int u = 0; u < BATCHES; ++u) {
-            const int64_t b = i * BATCHES + u;
+    for (int k = 0; k < 4; ++k) wo[k] = shuffle2(w[k], at.other);
+    const auto turn = [&](const Angles& a) {
+        a.get(at.low, cs, sn);
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                if (here(i, u) && h < at.heads) next[u * HEADS + h].load(x + b * s.xs[0] + h * s.xs[2]);
-                else next[u * HEADS + h].clear();
-            }
-            if (s.positions && here(i, u)) next_pos[u] = s.positions[(at.b0 + b) * s.tokens + at.token];
-        }
+        for (int k = 0; k < 4; ++k) cs[k] = mul2(cs[k], w[k]), sn[k] = mul2(sn[k], wo[k]);
     };
-    fetch(0);
-    for (int i = 0; i < rounds; ++i) {
-        F2 v[kRows][4];
-        int pos[BATCHES];
+    const auto work = [&](int i) {
+        Raw<T> raw[R::ROWS];
+        const uint4* rows = ring.round(i);
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) next[k].get(v[k]);
+        for (int k = 0; k < R::ROWS; ++k) raw[k].take(rows + k * Raw<T>::kPieces * kThreads);
+        ring.issue(i + R::kStages - 1);
 #pragma unroll
-        for (int u = 0; u < BATCHES; ++u) pos[u] = next_pos[u];
-        if (i + 1 < rounds) fetch(i + 1);
-#pragma unroll
-        for (int u = 0; u < BATCHES; ++u) {
-            if (s.positions) inside = angles(p, s, at, pos[u], cs, sn);
+        for (int u = 0; u < R::BATCHES; ++u) {
+            const int64_t b = i * R::BATCHES + u;
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
-                F2(&z)[4] = v[u * HEADS + h];
+                F2 z[4];
+                raw[u * HEADS + h].get(z);
                 F2 sum = mul2(z[0], z[0]);
 #pragma unroll
                 for (int k = 1; k < 4; ++k) sum = fma2(z[k], z[k], sum);
                 const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
                 const F2 r2 = pair(r, r);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) z[k] = mul2(mul2(z[k], r2), w[k]);
                 if (s.table) {
+                    F2 o[4];
+                    raw[u * HEADS + h].from(at.other).get(o);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const F2 o = shuffle2(z[k], at.other);
-                        z[k] = fma2(z[k], cs[k], mul2(o, sn[k]));
-                        if (!inside) z[k] = pair(NAN, NAN);
-                    }
+                    for (int k = 0; k < 4; ++k) z[k] = mul2(fma2(o[k], sn[k], mul2(z[k], cs[k])), r2);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) z[k] = mul2(mul2(z[k], r2), cs[k]);
                 }
-                if (h < at.heads && here(i, u)) Raw<T>::store(y + (i * BATCHES + u) * y_step + h * p.dim, z);
+                if (h < at.heads && at.b0 + b < at.b1) Raw<T>::store(y + b * y_step + h * p.dim, z);
             }
         }
+    };
+    if constexpr (POSITIONS) {
+        Positions<LANES, HEADS> positions(p, s, at);
+        for (int i = 0; i < rounds; ++i) {
+            turn(positions.next(i));
+            work(i);
+        }
+    } else {
+        if (s.table) {
+            Angles a;
+            a.load(p, s, at, at.token);
+            turn(a);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) cs[k] = w[k], sn[k] = pair(0.f, 0.f);
+        }
+        for (int i = 0; i < rounds; ++i) work(i);
     }
 }
 
-template <typename T, int LANES, int HEADS>
-__global__ void __launch_bounds__(kThreads) qk_norm_grad_kernel(const __grid_constant__ NormParams p)
+template <typename T, int LANES, int HEADS, bool POSITIONS>
+__global__ void __launch_bounds__(kThreads, 2) qk_norm_grad_kernel(const __grid_constant__ NormParams p)
 {
-    constexpr int BATCHES = kRows / HEADS;
-    __shared__ float sums[kThreads * 8];
+    using R = Ring<T, HEADS, 2, POSITIONS>;
+    extern __shared__ uint4 ring_memory[];
     const bool second = blockIdx.x >= p.side[0].blocks;
     const NormSide& s = p.side[second ? 1 : 0];
     const int block = second ? blockIdx.x - p.side[0].blocks : blockIdx.x;
     const Work<LANES, HEADS> at(p, s, block);
+    const int rounds = __reduce_max_sync(0xffffffffu, (at.b1 - at.b0 + R::BATCHES - 1) / R::BATCHES);
+    const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
+    const T* dy = static_cast<const T*>(s.dy) + at.b0 * s.ds[0] + at.token * s.ds[1] + at.h0 * s.ds[2] + at.sub * 8;
+    R ring{ring_memory + threadIdx.x, {x, dy}, {s.xs[0], s.ds[0]}, {s.xs[2], s.ds[2]}, at.b0, at.b1, at.heads};
+    ring.start();
+    const int64_t dx_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
+    T* dx = static_cast<T*>(s.y) + at.b0 * dx_step + (static_cast<int64_t>(at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
+
     F2 w[4], dw[4], cs[4], sn[4];
     load_weight(w, s, at.sub, at.active);
 #pragma unroll
     for (int k = 0; k < 4; ++k) dw[k] = pair(0.f, 0.f);
-    bool inside = true;
-    if (s.table && !s.positions) inside = angles(p, s, at, at.token, cs, sn);
-
-    const int rounds = __reduce_max_sync(0xffffffffu, (at.b1 - at.b0 + BATCHES - 1) / BATCHES);
-    const T* x = static_cast<const T*>(s.x) + at.b0 * s.xs[0] + at.token * s.xs[1] + at.h0 * s.xs[2] + at.sub * 8;
-    const T* dy = static_cast<const T*>(s.dy) + at.b0 * s.ds[0] + at.token * s.ds[1] + at.h0 * s.ds[2] + at.sub * 8;
-    const int64_t dx_step = static_cast<int64_t>(s.tokens) * s.heads * p.dim;
-    T* dx = static_cast<T*>(s.y) + at.b0 * dx_step + (static_cast<int64_t>(at.token) * s.heads + at.h0) * p.dim + at.sub * 8;
-    for (int i = 0; i < rounds; ++i) {
-        Raw<T> rx[kRows], rg[kRows];
-        int pos[BATCHES];
+    const auto work = [&](int i) {
+        Raw<T> rx[R::ROWS], rg[R::ROWS];
+        const uint4* rows = ring.round(i);
 #pragma unroll
-        for (int u = 0; u < BATCHES; ++u) {
-            const int64_t b = i * BATCHES + u;
-            const bool on = at.b0 + b < at.b1;
-            pos[u] = at.token;
-            if (s.positions && on) pos[u] = s.positions[(at.b0 + b) * s.tokens + at.token];
-#pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                const int k = u * HEADS + h;
-                if (on && h < at.heads) {
-                    rx[k].load(x + b * s.xs[0] + h * s.xs[2]);
-                    rg[k].load(dy + b * s.ds[0] + h * s.ds[2]);
-                } else {
-                    rx[k].clear();
-                    rg[k].clear();
-                }
-            }
+        for (int k = 0; k < R::ROWS; ++k) {
+            rx[k].take(rows + k * Raw<T>::kPieces * kThreads);
+            rg[k].take(rows + (R::ROWS + k) * Raw<T>::kPieces * kThreads);
         }
+        ring.issue(i + R::kStages - 1);
 #pragma unroll
-        for (int u = 0; u < BATCHES; ++u) {
-            const int64_t b = i * BATCHES + u;
-            if (s.positions) inside = angles(p, s, at, pos[u], cs, sn);
+        for (int u = 0; u < R::BATCHES; ++u) {
+            const int64_t b = i * R::BATCHES + u;
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
-                const bool here = at.b0 + b < at.b1 && h < at.heads;
-                F2 v[4], g[4];
+                F2 v[4], g[4], gw[4];
                 rx[u * HEADS + h].get(v);
                 rg[u * HEADS + h].get(g);
-                if (s.table) {  // the rotation back: the sines change sign
+                if (s.table) {
+                    F2 o[4];
+                    rg[u * HEADS + h].from(at.other).get(o);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const F2 o = shuffle2(g[k], at.other);
-                        g[k] = fma2(g[k], cs[k], mul2(mul2(o, sn[k]), pair(-1.f, -1.f)));
-                        if (!inside && here) g[k] = pair(NAN, NAN);
-                    }
+                    for (int k = 0; k < 4; ++k) g[k] = fma2(o[k], sn[k], mul2(g[k], cs[k]));
                 }
-                F2 sum = mul2(v[0], v[0]), dot = mul2(mul2(v[0], w[0]), g[0]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) gw[k] = mul2(g[k], w[k]);
+                F2 sum = mul2(v[0], v[0]), dot = mul2(v[0], gw[0]);
 #pragma unroll
                 for (int k = 1; k < 4; ++k) {
                     sum = fma2(v[k], v[k], sum);
-                    dot = fma2(mul2(v[k], w[k]), g[k], dot);
+                    dot = fma2(v[k], gw[k], dot);
                 }
                 const float r = rsqrtf(fmaf(row_sum<LANES>(sum), p.inv_dim, p.eps));
                 const float f = -r * r * r * (row_sum<LANES>(dot) * p.inv_dim);
                 const F2 r2 = pair(r, r), f2 = pair(f, f);
-                if (here) {
+                if (h < at.heads && at.b0 + b < at.b1) {
                     F2 d[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const F2 gr = mul2(g[k], r2);
-                        dw[k] = fma2(gr, v[k], dw[k]);
-                        d[k] = fma2(gr, w[k], mul2(f2, v[k]));
+                        dw[k] = fma2(mul2(g[k], r2), v[k], dw[k]);
+                        d[k] = fma2(gw[k], r2, mul2(f2, v[k]));
                     }
                     Raw<T>::store(dx + b * dx_step + h * p.dim, d);
                 }
             }
         }
+    };
+    // the rotation back: the sines change sign
+    if constexpr (POSITIONS) {
+        Positions<LANES, HEADS> positions(p, s, at);
+        for (int i = 0; i < rounds; ++i) {
+            positions.next(i).get(!at.low, cs, sn);
+            work(i);
+        }
+    } else {
+        if (s.table) {
+            Angles a;
+            a.load(p, s, at, at.token);
+            a.get(!at.low, cs, sn);
+        }
+        for (int i = 0; i < rounds; ++i) work(i);
     }
     if (!s.part) return;
+    copy_wait<0>();
+    __syncthreads();
     // the block's rows, in order
+    float* sums = reinterpret_cast<float*>(ring_memory);
+    static_assert(R::kBytes >= sizeof(float) * kThreads * 8, "the ring holds the sums");
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float2 f = both(dw[k]);
@@ -443,16 +564,15 @@ struct NormShape {
 
 NormShape norm_shape(const policy_qk_norm& a)
 {
-    NormShape s{4, 4};
+    NormShape s{4, a.dtype == POLICY_F32 ? kRows<float> : kRows<bf16>};
     while (s.lanes * 8 < a.dim) s.lanes *= 2;
     const policy_norm_side& big = a.side[0].tokens * a.side[0].heads > a.side[1].tokens * a.side[1].heads ? a.side[0] : a.side[1];
-    if (big.heads <= 2) s.heads = big.heads;
+    if (big.heads < s.heads && big.heads <= 2) s.heads = big.heads;
     return s;
 }
 
-// Threads' ranges of batches: as long as they leave the device kRounds full sets of blocks.
+// Threads' ranges of batches: as long as they leave each SM this many blocks.
 constexpr int kBlocksPerSm = 8;
-constexpr int kRounds = 2;
 
 int make_norm(const policy_qk_norm& a, int sms, bool backward, NormParams& p)
 {
@@ -473,8 +593,8 @@ int make_norm(const policy_qk_norm& a, int sms, bool backward, NormParams& p)
         d.chunks = (s.heads + shape.heads - 1) / shape.heads;
         total += a.batch * s.tokens * d.chunks;
     }
-    const int64_t want = static_cast<int64_t>(sms) * kBlocksPerSm * kRounds * groups;
-    const int64_t round = kRows / shape.heads;  // batches at a time
+    const int64_t want = static_cast<int64_t>(sms) * kBlocksPerSm * groups;
+    const int64_t round = (a.dtype == POLICY_F32 ? kRows<float> : kRows<bf16>) / shape.heads;  // batches at a time
     const int64_t length = total / want > 1 ? (total / want + round - 1) / round * round : 1;  // batches of a thread
     for (NormSide& d : p.side) {
         d.splits = static_cast<int>((a.batch + length - 1) / length);
@@ -485,28 +605,52 @@ int make_norm(const policy_qk_norm& a, int sms, bool backward, NormParams& p)
     return POLICY_OK;
 }
 
-template <typename T, int LANES, int HEADS>
-void launch_norm(const NormParams& p, bool backward, unsigned blocks, cudaStream_t stream)
+template <typename K>
+int launch_ring(K kernel, size_t bytes, const NormParams& p, unsigned blocks, int device, std::atomic<uint64_t>& done, cudaStream_t stream)
 {
-    if (backward) qk_norm_grad_kernel<T, LANES, HEADS><<<blocks, kThreads, 0, stream>>>(p);
-    else qk_norm_kernel<T, LANES, HEADS><<<blocks, kThreads, 0, stream>>>(p);
+    const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+    if (!bit || !(done.load(std::memory_order_relaxed) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    kernel<<<blocks, kThreads, bytes, stream>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? POLICY_OK : cuda_fail(e, "qk_norm_kernel");
+}
+
+template <typename T, int LANES, int HEADS, bool POSITIONS>
+int launch_norm(const NormParams& p, bool backward, unsigned blocks, int device, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> done{0}, done_grad{0};
+    if (backward)
+        return launch_ring(qk_norm_grad_kernel<T, LANES, HEADS, POSITIONS>, Ring<T, HEADS, 2, POSITIONS>::kBytes, p, blocks, device, done_grad, stream);
+    return launch_ring(qk_norm_kernel<T, LANES, HEADS, POSITIONS>, Ring<T, HEADS, 1, POSITIONS>::kBytes, p, blocks, device, done, stream);
+}
+
+template <typename T, int LANES, int HEADS>
+int launch_norm(const NormParams& p, bool backward, unsigned blocks, int device, cudaStream_t stream)
+{
+    if (p.side[0].positions || p.side[1].positions) return launch_norm<T, LANES, HEADS, true>(p, backward, blocks, device, stream);
+    return launch_norm<T, LANES, HEADS, false>(p, backward, blocks, device, stream);
 }
 
 template <typename T, int LANES>
-void launch_norm(const NormParams& p, int heads, bool backward, unsigned blocks, cudaStream_t stream)
+int launch_norm(const NormParams& p, int heads, bool backward, unsigned blocks, int device, cudaStream_t stream)
 {
-    if (heads == 1) launch_norm<T, LANES, 1>(p, backward, blocks, stream);
-    else if (heads == 2) launch_norm<T, LANES, 2>(p, backward, blocks, stream);
-    else launch_norm<T, LANES, 4>(p, backward, blocks, stream);
+    if (heads == 1) return launch_norm<T, LANES, 1>(p, backward, blocks, device, stream);
+    if (sizeof(T) == 4 || heads == 2) return launch_norm<T, LANES, 2>(p, backward, blocks, device, stream);
+    if constexpr (sizeof(T) == 2) return launch_norm<T, LANES, 4>(p, backward, blocks, device, stream);
+    return POLICY_ERR_INVALID;
 }
 
 template <typename T>
-void launch_norm(const NormParams& p, const NormShape& s, bool backward, unsigned blocks, cudaStream_t stream)
+int launch_norm(const NormParams& p, const NormShape& s, bool backward, unsigned blocks, int device, cudaStream_t stream)
 {
-    if (s.lanes == 4) launch_norm<T, 4>(p, s.heads, backward, blocks, stream);
-    else if (s.lanes == 8) launch_norm<T, 8>(p, s.heads, backward, blocks, stream);
-    else if (s.lanes == 16) launch_norm<T, 16>(p, s.heads, backward, blocks, stream);
-    else launch_norm<T, 32>(p, s.heads, backward, blocks, stream);
+    if (s.lanes == 4) return launch_norm<T, 4>(p, s.heads, backward, blocks, device, stream);
+    if (s.lanes == 8) return launch_norm<T, 8>(p, s.heads, backward, blocks, device, stream);
+    if (s.lanes == 16) return launch_norm<T, 16>(p, s.heads, backward, blocks, device, stream);
+    return launch_norm<T, 32>(p, s.heads, backward, blocks, device, stream);
 }
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -537,10 +681,9 @@ int run_norm(const policy_qk_norm* a, bool backward, cudaStream_t stream)
     }
     if (blocks > 0) {
         const NormShape shape = norm_shape(*a);
-        if (a->dtype == POLICY_F32) launch_norm<float>(p, shape, backward, blocks, stream);
-        else launch_norm<bf16>(p, shape, backward, blocks, stream);
-        const cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess) return cuda_fail(e, "qk_norm_kernel");
+        rc = a->dtype == POLICY_F32 ? launch_norm<float>(p, shape, backward, blocks, a->device, stream)
+                                    : launch_norm<bf16>(p, shape, backward, blocks, a->device, stream);
+        if (rc != POLICY_OK) return rc;
     }
     if (weights) {
         norm_weight_kernel<<<dim3(p.dim / 8, 2), 1024, 0, stream>>>(p);
