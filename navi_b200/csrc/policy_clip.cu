@@ -3,8 +3,9 @@
 // Two launches: every block adds the squares of its chunks (32 bits within a thread's chunk, 64 bits
 // from there on) into one partial sum; every block of the second launch adds the partial sums in the
 // same order, which costs it a few kilobytes from L2 and saves a launch between the two, and scales
-// its chunks.  Memory bounds both; the second pass takes the chunks in the opposite order, so that it
-// starts on what the first left in L2.
+// its chunks.  The second launch starts while the first still runs (programmatic dependent launch): its
+// blocks read their first chunk before they wait for the partial sums.  Memory bounds both; the second pass
+// takes the chunks in the opposite order, so that it starts on what the first left in L2.
 #include <cuda_bf16.h>
 
 #include <limits>
@@ -17,7 +18,8 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int kThreads = 256;
-constexpr int kChunk = 8192;        // values: 32 per thread, all in flight at once
+// Values of a chunk: 32 per thread where there are chunks enough for every SM, else 8.
+constexpr int kLongChunk = 8192, kShortChunk = 2048;
 constexpr int kBlocksPerSm = 8;     // 256 threads: the SM is full
 constexpr int kMaxSms = 256;         // SMs that the workspace allows for
 constexpr int kTensors = 512;       // tensors of one launch (its parameters: 16 KB)
@@ -31,7 +33,7 @@ struct ClipTensor {
     uint32_t dtype;        // bit 0: bf16; bit 1: every chunk is 16-byte aligned
 };
 
-template <int N>
+template <int N, int CHUNK>
 struct ClipParams {
     ClipTensor t[N];
     double* parts;
@@ -43,8 +45,8 @@ struct ClipParams {
     int n_parts; // all partial sums (second pass)
 };
 
-template <int N>
-__device__ __forceinline__ int find_tensor(const ClipParams<N>& p, uint32_t chunk)
+template <int N, int CHUNK>
+__device__ __forceinline__ int find_tensor(const ClipParams<N, CHUNK>& p, uint32_t chunk)
 {
     int lo = 0, hi = p.n - 1;
     while (lo < hi) {
@@ -84,95 +86,116 @@ __device__ __forceinline__ uint32_t scale2(uint32_t w, float c)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_constant__ ClipParams<N> p)
-{
-    double sum = 0.0;
-    for (uint32_t chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
-        const ClipTensor& t = p.t[find_tensor(p, chunk)];
-        const uint64_t at = static_cast<uint64_t>(chunk - t.first_chunk) * kChunk;
-        const int n = static_cast<int>(min(static_cast<uint64_t>(kChunk), t.count - at));
+// One chunk of a tensor, in registers where it is whole and aligned.
+template <int N, int CHUNK>
+struct Chunk {
+    static constexpr int kWords = CHUNK / kThreads / 4;  // 16-byte words of f32; half as many of bf16
+    const ClipTensor* t;
+    uint64_t at;
+    int n;
+    bool wide;
+    uint4 v[kWords];
+
+    __device__ __forceinline__ void load(const ClipParams<N, CHUNK>& p, uint32_t chunk)
+    {
+        t = &p.t[find_tensor(p, chunk)];
+        at = static_cast<uint64_t>(chunk - t->first_chunk) * CHUNK;
+        n = static_cast<int>(min(static_cast<uint64_t>(CHUNK), t->count - at));
+        wide = n == CHUNK && (t->dtype & 2u);
+        if (!wide) return;
+        if (t->dtype & 1u) {
+            const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t->grad) + at);
+#pragma unroll
+            for (int i = 0; i < kWords / 2; ++i) v[i] = g[threadIdx.x + i * kThreads];
+        } else {
+            const uint4* g = reinterpret_cast<const uint4*>(static_cast<const float*>(t->grad) + at);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) v[i] = g[threadIdx.x + i * kThreads];
+        }
+    }
+    __device__ __forceinline__ float value(int i) const
+    {
+        return (t->dtype & 1u) ? __bfloat162float(static_cast<const bf16*>(t->grad)[at + i]) : static_cast<const float*>(t->grad)[at + i];
+    }
+    __device__ __forceinline__ float squares() const
+    {
         float x = 0.f;
-        if (n == kChunk && (t.dtype & 2u)) {
-            if (t.dtype & 1u) {
-                const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.grad) + at);
-                uint4 v[4];
+        if (!wide) {
+            for (int i = threadIdx.x; i < n; i += kThreads) x = fmaf(value(i), value(i), x);
+        } else if (t->dtype & 1u) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
+            for (int i = 0; i < kWords / 2; ++i) {
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 f = unpack(w[k]);
-                        x = fmaf(f.x, f.x, fmaf(f.y, f.y, x));
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = unpack(w[k]);
+                    x = fmaf(f.x, f.x, fmaf(f.y, f.y, x));
                 }
-            } else {
-                const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
-                float4 v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = g[threadIdx.x + i * kThreads];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x = fmaf(v[i].x, v[i].x, fmaf(v[i].y, v[i].y, fmaf(v[i].z, v[i].z, fmaf(v[i].w, v[i].w, x))));
             }
         } else {
-            for (int i = threadIdx.x; i < n; i += kThreads) {
-                const float v = (t.dtype & 1u) ? __bfloat162float(static_cast<const bf16*>(t.grad)[at + i])
-                                               : static_cast<const float*>(t.grad)[at + i];
-                x = fmaf(v, v, x);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const float4 f = make_float4(__uint_as_float(v[i].x), __uint_as_float(v[i].y), __uint_as_float(v[i].z), __uint_as_float(v[i].w));
+                x = fmaf(f.x, f.x, fmaf(f.y, f.y, fmaf(f.z, f.z, fmaf(f.w, f.w, x))));
             }
         }
-        sum += x;
+        return x;
+    }
+    __device__ __forceinline__ void scale(float c) const
+    {
+        if (c == 1.f && t->out == t->grad) return;
+        if (!wide) {
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                if (t->dtype & 1u) static_cast<bf16*>(t->out)[at + i] = __float2bfloat16_rn(value(i) * c);
+                else static_cast<float*>(t->out)[at + i] = value(i) * c;
+            }
+        } else if (t->dtype & 1u) {
+            uint4* o = reinterpret_cast<uint4*>(static_cast<bf16*>(t->out) + at);
+#pragma unroll
+            for (int i = 0; i < kWords / 2; ++i)
+                o[threadIdx.x + i * kThreads] = make_uint4(scale2(v[i].x, c), scale2(v[i].y, c), scale2(v[i].z, c), scale2(v[i].w, c));
+        } else {
+            float4* o = reinterpret_cast<float4*>(static_cast<float*>(t->out) + at);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                o[threadIdx.x + i * kThreads] = make_float4(__uint_as_float(v[i].x) * c, __uint_as_float(v[i].y) * c, __uint_as_float(v[i].z) * c,
+                                                            __uint_as_float(v[i].w) * c);
+        }
+    }
+};
+
+template <int N, int CHUNK>
+__global__ void __launch_bounds__(kThreads) clip_norm_kernel(const __grid_constant__ ClipParams<N, CHUNK> p)
+{
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    double sum = 0.0;
+    Chunk<N, CHUNK> c;
+    for (uint32_t chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
+        c.load(p, chunk);
+        sum += c.squares();
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) p.parts[p.part0 + blockIdx.x] = sum;
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ ClipParams<N> p)
+template <int N, int CHUNK>
+__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ ClipParams<N, CHUNK> p)
 {
+    Chunk<N, CHUNK> c;
+    uint32_t k = blockIdx.x;
+    c.load(p, p.chunks - 1 - k);
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     double sum = 0.0;
     for (int i = threadIdx.x; i < p.n_parts; i += kThreads) sum += p.parts[i];
     const float norm = static_cast<float>(sqrt(block_sum(sum)));
     if (p.norm && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = norm;
     const float f = p.max_norm / (norm + 1e-6f);
-    const float c = f > 1.f ? 1.f : f;  // NaN stays NaN
-    for (uint32_t k = blockIdx.x; k < p.chunks; k += gridDim.x) {
-        const uint32_t chunk = p.chunks - 1 - k;
-        const ClipTensor& t = p.t[find_tensor(p, chunk)];
-        if (c == 1.f && t.out == t.grad) continue;
-        const uint64_t at = static_cast<uint64_t>(chunk - t.first_chunk) * kChunk;
-        const int n = static_cast<int>(min(static_cast<uint64_t>(kChunk), t.count - at));
-        if (n == kChunk && (t.dtype & 2u)) {
-            if (t.dtype & 1u) {
-                const uint4* g = reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.grad) + at);
-                uint4* o = reinterpret_cast<uint4*>(static_cast<bf16*>(t.out) + at);
-                uint4 v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = g[threadIdx.x + i * kThreads];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    o[threadIdx.x + i * kThreads] = make_uint4(scale2(v[i].x, c), scale2(v[i].y, c), scale2(v[i].z, c), scale2(v[i].w, c));
-            } else {
-                const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(t.grad) + at);
-                float4* o = reinterpret_cast<float4*>(static_cast<float*>(t.out) + at);
-                float4 v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = g[threadIdx.x + i * kThreads];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    o[threadIdx.x + i * kThreads] = make_float4(v[i].x * c, v[i].y * c, v[i].z * c, v[i].w * c);
-            }
-        } else {
-            for (int i = threadIdx.x; i < n; i += kThreads) {
-                if (t.dtype & 1u)
-                    static_cast<bf16*>(t.out)[at + i] = __float2bfloat16_rn(__bfloat162float(static_cast<const bf16*>(t.grad)[at + i]) * c);
-                else
-                    static_cast<float*>(t.out)[at + i] = static_cast<const float*>(t.grad)[at + i] * c;
-            }
-        }
+    const float factor = f > 1.f ? 1.f : f;  // NaN stays NaN
+    for (;;) {
+        c.scale(factor);
+        k += gridDim.x;
+        if (k >= p.chunks) break;
+        c.load(p, p.chunks - 1 - k);
     }
 }
 
@@ -195,8 +218,8 @@ int check_grads(const policy_grad* grads, int64_t n)
 }
 
 // Takes tensors from grads[i..] for one launch; returns how many entries it consumed.
-template <int N>
-int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams<N>& p)
+template <int N, int CHUNK>
+int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams<N, CHUNK>& p)
 {
     p.n = 0;
     uint64_t chunks = 0;
@@ -204,7 +227,7 @@ int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams<N>& p)
     for (; i < n && p.n < N; ++i) {
         const policy_grad& g = grads[i];
         if (g.count == 0) continue;
-        const uint64_t own = (g.count + kChunk - 1) / kChunk;
+        const uint64_t own = (g.count + CHUNK - 1) / CHUNK;
         if (chunks + own > std::numeric_limits<int32_t>::max()) break;  // one tensor alone always fits: count <= 2^40
         ClipTensor& t = p.t[p.n++];
         const bool wide = reinterpret_cast<uintptr_t>(g.grad) % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
@@ -217,20 +240,21 @@ int64_t fill_launch(const policy_grad* grads, int64_t n, ClipParams<N>& p)
     return i;
 }
 
-template <int N>
-int launch_blocks(const ClipParams<N>& p, int sms)
+template <int N, int CHUNK>
+int launch_blocks(const ClipParams<N, CHUNK>& p, int sms)
 {
     const uint32_t most = static_cast<uint32_t>(sms < kMaxSms ? sms : kMaxSms) * kBlocksPerSm;
     return static_cast<int>(p.chunks < most ? p.chunks : most);
 }
 
-template <int N>
+template <int N, int CHUNK>
 int launch_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, int sms, void* workspace, cudaStream_t stream)
 {
-    ClipParams<N> p;
+    ClipParams<N, CHUNK> p;
     p.parts = static_cast<double*>(workspace);
     p.max_norm = max_norm;
     p.n_parts = 0;
+    bool one_launch = false;
     for (int64_t i = 0; i < n;) {
         i += fill_launch(grads + i, n - i, p);
         if (p.chunks == 0) continue;
@@ -240,6 +264,7 @@ int launch_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm
         clip_norm_kernel<<<blocks, kThreads, 0, stream>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "clip_norm_kernel");
+        one_launch = p.n_parts == 0;
         p.n_parts += blocks;
     }
     if (p.n_parts == 0) {
@@ -247,12 +272,21 @@ int launch_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm
         return e == cudaSuccess ? POLICY_OK : cuda_fail(e, "cudaMemsetAsync");
     }
     p.norm = norm;
+    // With several launches the first scaling one may start only when every sum is written, which the launch
+    // before it alone does not say; the gradients of a later one are not read before it starts.
+    bool first = one_launch;
     for (int64_t i = 0; i < n;) {
         i += fill_launch(grads + i, n - i, p);
         if (p.chunks == 0) continue;
-        clip_scale_kernel<<<launch_blocks(p, sms), kThreads, 0, stream>>>(p);
-        const cudaError_t e = cudaGetLastError();
+        cudaLaunchAttribute early{};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = first;
+        cudaLaunchConfig_t config{};
+        config.gridDim = launch_blocks(p, sms), config.blockDim = kThreads, config.stream = stream;
+        config.attrs = &early, config.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&config, clip_scale_kernel<N, CHUNK>, p);
         if (e != cudaSuccess) return cuda_fail(e, "clip_scale_kernel");
+        first = false;
         p.norm = nullptr;
     }
     return POLICY_OK;
@@ -268,8 +302,14 @@ int run_clip(const policy_grad* grads, int64_t n, float max_norm, float* norm, i
     if (info.status != POLICY_OK) return info.status;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return cuda_fail(scope.error(), "cudaSetDevice");
-    if (n <= kFewTensors) return launch_clip<kFewTensors>(grads, n, max_norm, norm, info.sms, workspace, stream);
-    return launch_clip<kTensors>(grads, n, max_norm, norm, info.sms, workspace, stream);
+    uint64_t values = 0;
+    for (int64_t i = 0; i < n; ++i) values += grads[i].count;
+    const bool few = values < static_cast<uint64_t>(info.sms) * 4 * kLongChunk;
+    if (n <= kFewTensors)
+        return few ? launch_clip<kFewTensors, kShortChunk>(grads, n, max_norm, norm, info.sms, workspace, stream)
+                   : launch_clip<kFewTensors, kLongChunk>(grads, n, max_norm, norm, info.sms, workspace, stream);
+    return few ? launch_clip<kTensors, kShortChunk>(grads, n, max_norm, norm, info.sms, workspace, stream)
+               : launch_clip<kTensors, kLongChunk>(grads, n, max_norm, norm, info.sms, workspace, stream);
 }
 
 }  // namespace
