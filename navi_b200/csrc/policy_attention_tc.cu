@@ -43,8 +43,6 @@ struct TcShape {
     static constexpr int kStages = DP == 64 ? 3 : 2;
     // columns of tensor memory
     static constexpr bool kApart = DP == 64;
-    // P is handed over in halves of its keys at dim 64 (3 % at 4,096 x 768); at dim 128 in one (2 % at 12,288 x 768)
-    static constexpr int kHalves = kApart ? 2 : 1;
     static constexpr int kOutputs = 2 * kTile, kWeights = kApart ? kOutputs + 2 * DP : 0, kWeightStep = kApart ? kTile / 2 : kTile;
     static constexpr uint32_t kQ = 0;
     static constexpr uint32_t kK = 2 * kTileBytes;
@@ -263,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok || !(ok = bar_wait(bar(v_ready + st), (uses / ST) & 1u, broken))) break;
                     // the item before has left O
                     if (t == item.t0 && !(ok = bar_wait(bar(kOEmpty + i), (items_done & 1u) ^ 1u, broken))) break;
-                    constexpr int kSteps = kTile / 16 / S::kHalves;
-                    for (int half = 0; half < S::kHalves && ok; ++half) {
+                    constexpr int kSteps = kTile / 16 / 2;
+                    for (int half = 0; half < 2 && ok; ++half) {
                         if (!(ok = bar_wait(bar(kPFull + 2 * i + half), tiles_done & 1u, broken))) break;
                         fence_after_sync();
                         const uint32_t v = values_at + st * (S::kTileBytes >> 4) + half * kSteps * (16 * kBlockRow >> 4);
@@ -351,9 +349,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = warp_wait(bar(kSFull + i), score_uses & 1u, broken))) break;
                 ++score_uses;
                 fence_after_sync();
-                float s[kTile];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) tmem_load32(s + q * 32, ts + q * 32);
+                // S is read twice, 32 columns ahead of the work: for the maximum, and for the weights.  A whole row in
+                // registers spilled, and was 17 % slower at dim 128.
+                float s[64];
+                tmem_load32(s, ts);
                 int ahead = items;
                 if (t + 1 == item.t1) {
                     ahead = next_item(it + gridDim.x);
@@ -377,23 +376,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 float x[4] = {top, top, top, top};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int q = 0; q < 4; ++q) {
+                    float* now = s + (q & 1) * 32;
                     tmem_wait_load();
-                    if (h == 0) {
-                        tmem_load32(s + 64, ts + 64);
-                        tmem_load32(s + 96, ts + 96);
-                    } else if (S::kApart) {
-                        fence_before_sync();
-                        warp_arrive(bar(kSFree + i));
-                    }
+                    if (q < 3) tmem_load32(s + ((q + 1) & 1) * 32, ts + (q + 1) * 32);
                     if (!whole) {
 #pragma unroll
-                        for (int j = h * 64; j < h * 64 + 64; ++j)
-                            if (!((vis[j >> 5] >> (j & 31)) & 1u)) s[j] = -INFINITY;
+                        for (int j = 0; j < 32; ++j)
+                            if (!((vis[q] >> j) & 1u)) now[j] = -INFINITY;
+                        tmem_store32(ts + q * 32, now);
                     }
 #pragma unroll
-                    for (int j = h * 64; j < h * 64 + 64; j += 2) x[(j >> 1) & 3] = fmaxf(x[(j >> 1) & 3], fmaxf(s[j], s[j + 1]));
+                    for (int j = 0; j < 32; j += 2) x[(j >> 1) & 3] = fmaxf(x[(j >> 1) & 3], fmaxf(now[j], now[j + 1]));
                 }
+                if (!whole) tmem_wait_store();
+                tmem_load32(s, ts);
                 top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                 if (S::kApart && score_uses > 1) {  // the products with the weights before these are over
                     if (!(ok = warp_wait(bar(kPFree + i), (score_uses & 1u), broken))) break;
@@ -430,18 +427,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t w[16];
+                    float* now = s + (q & 1) * 32;
+                    tmem_wait_load();
+                    if (q < 3) {
+                        tmem_load32(s + ((q + 1) & 1) * 32, ts + (q + 1) * 32);
+                    } else if (S::kApart) {
+                        fence_before_sync();
+                        warp_arrive(bar(kSFree + i));
+                    }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        float2 e = fma2(make_float2(s[q * 32 + 2 * j], s[q * 32 + 2 * j + 1]), c2, b2);
+                        float2 e = fma2(make_float2(now[2 * j], now[2 * j + 1]), c2, b2);
                         e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                         sum = add2(sum, e);
                         w[j] = Mma<bf16>::pack(e.x, e.y);
                     }
                     tmem_store16(tp + q * 16, w);
-                    if (S::kHalves == 2 ? q & 1 : q == 3) {
+                    if (q & 1) {
                         tmem_wait_store();
                         fence_before_sync();
-                        warp_arrive(bar(kPFull + 2 * i + (S::kHalves == 2 ? q >> 1 : 0)));
+                        warp_arrive(bar(kPFull + 2 * i + (q >> 1)));
                     }
                 }
                 if (both) warp_arrive(bar(kTurn + (warp ^ 4)));
