@@ -98,14 +98,35 @@ struct KeyLoader {
 
 // c += a b over the k steps; f32 sums the tile apart and adds it rounded to nearest, since the
 // tensor core truncates every accumulation and a long chain of truncations is a bias
-template <typename T, int STEPS, typename LoadB>
-__device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const typename Mma<T>::A (&a)[STEPS], LoadB&& load)
+//
+// f32 also leaves out the steps and columns that hold nothing but the padding of the dim, of the last key tile or of
+// the last row tile (`used` of STEPS here, the same for the whole warp): its three products and the splitting make
+// them dear, 33 % at dim 96 and most of the time at 3 keys.  Tiles without padding run code without these
+// branches, which keep steps from overlapping (20 % at dim 64).
+template <bool V>
+struct Flag {
+    static constexpr bool value = V;
+};
+template <typename T, typename F>
+__device__ __forceinline__ void with_padding(bool padded, F&& f)
+{
+    if constexpr (Mma<T>::kExact) {
+        if (padded) f(Flag<true>{});
+        else f(Flag<false>{});
+    } else {
+        f(Flag<false>{});
+    }
+}
+
+template <typename T, int STEPS, bool PADDED, typename LoadB>
+__device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const typename Mma<T>::A (&a)[STEPS], int used, LoadB&& load)
 {
     using M = Mma<T>;
     if constexpr (M::kExact) {
         float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < STEPS; ++kk) {
+            if (PADDED && kk >= used) break;
             typename M::B b0, b1;
             load(b0, b1, kk);
             M::mma(t0, a[kk], b0);
@@ -128,15 +149,16 @@ __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const
 // and then rounds to nearest, for the same reason.
 constexpr int kFlush = 4;
 
-template <typename T, int STEPS, int N, typename Step>
-__device__ __forceinline__ void multiply(float (&c)[N][4], Step&& step)
+template <typename T, int STEPS, bool PADDED, int N, typename Step>
+__device__ __forceinline__ void multiply(float (&c)[N][4], int dim, Step&& step)
 {
     if constexpr (Mma<T>::kExact) {
 #pragma unroll
         for (int k0 = 0; k0 < STEPS; k0 += kFlush) {
             float t[N][4] = {};
 #pragma unroll
-            for (int kk = k0; kk < k0 + kFlush && kk < STEPS; ++kk) step(t, kk);
+            for (int kk = k0; kk < k0 + kFlush && kk < STEPS; ++kk)
+                if (!PADDED || kk * Mma<T>::KS < dim) step(t, kk);
 #pragma unroll
             for (int j = 0; j < N; ++j)
 #pragma unroll
@@ -230,17 +252,22 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
         for (int j = 0; j < KSL / 8; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
-        multiply<T, STEPS>(s, [&](float (&t)[KSL / 8][4], int kk) {
-            typename M::A a;
-            if constexpr (QREG) a = qf[kk];
-            else M::load_a(a, sq + wm * 16 * PITCH + kk * KS, PITCH, lane);
+        const int left = min(n - t * KT, KT) - wn * KSL;  // keys of this warp's part of the tile
+        const bool padded = p.dim < DP || left < KSL;
+        with_padding<T>(padded, [&](auto pad) {
+            multiply<T, STEPS, pad.value>(s, p.dim, [&](float (&x)[KSL / 8][4], int kk) {
+                typename M::A a;
+                if constexpr (QREG) a = qf[kk];
+                else M::load_a(a, sq + wm * 16 * PITCH + kk * KS, PITCH, lane);
 #pragma unroll
-            for (int j = 0; j < KSL / 16; ++j) {
-                typename M::B b0, b1;
-                M::load_b_nk(b0, b1, tk + j * 16 * PITCH + kk * KS, PITCH, lane);
-                M::mma(t[2 * j], a, b0);
-                M::mma(t[2 * j + 1], a, b1);
-            }
+                for (int j = 0; j < KSL / 16; ++j) {
+                    if (pad.value && j * 16 >= left) break;
+                    typename M::B b0, b1;
+                    M::load_b_nk(b0, b1, tk + j * 16 * PITCH + kk * KS, PITCH, lane);
+                    M::mma(x[2 * j], a, b0);
+                    M::mma(x[2 * j + 1], a, b1);
+                }
+            });
         });
         if (p.mask || (t + 1) * KT > n) {
             const uint8_t* vis = svis + st * KT + wn * KSL + (lane & 3) * 2;
@@ -274,17 +301,20 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
         typename M::A pf[KSL / KS];
 #pragma unroll
         for (int kk = 0; kk < KSL / KS; ++kk) M::from_c(pf[kk], s, kk);
+        with_padding<T>(padded, [&](auto pad) {
 #pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
+            for (int j = 0; j < DP / 16; ++j) {
+                if (pad.value && j * 16 >= p.dim) break;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                o[2 * j + h][0] *= a0, o[2 * j + h][1] *= a0;
-                o[2 * j + h][2] *= a1, o[2 * j + h][3] *= a1;
+                for (int h = 0; h < 2; ++h) {
+                    o[2 * j + h][0] *= a0, o[2 * j + h][1] *= a0;
+                    o[2 * j + h][2] *= a1, o[2 * j + h][3] *= a1;
+                }
+                accumulate<T, KSL / KS, pad.value>(o[2 * j], o[2 * j + 1], pf, (left + KS - 1) / KS, [&](typename M::B& b0_, typename M::B& b1_, int kk) {
+                    M::load_b_kn(b0_, b1_, tv + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
             }
-            accumulate<T, KSL / KS>(o[2 * j], o[2 * j + 1], pf, [&](typename M::B& b0_, typename M::B& b1_, int kk) {
-                M::load_b_kn(b0_, b1_, tv + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-        }
+        });
     }
 
     // the warps along the keys meet in shared memory, and the rows leave it in whole vectors
@@ -534,18 +564,22 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
         T* tk = sk + (st * KT + warp * 16) * PITCH;
         T* tv = sv + (st * KT + warp * 16) * PITCH;
         float s[2][4] = {}, dp[2][4] = {};  // [16 keys] x [16 rows]
-        const auto product = [&](float (&out)[2][4], const T* a_tile, const T* b_tile) {
-            multiply<T, STEPS>(out, [&](float (&x)[2][4], int kk) {
-                typename M::A a;
-                typename M::B b0, b1;
-                M::load_a(a, a_tile + kk * KS, PITCH, lane);
-                M::load_b_nk(b0, b1, b_tile + kk * KS, PITCH, lane);
-                M::mma(x[0], a, b0);
-                M::mma(x[1], a, b1);
-            });
-        };
-        product(s, tk, sq);
-        product(dp, tv, sdo);
+        const bool live = t * KT + warp * 16 < n;  // some key of the warp's may be visible
+        const bool padded = !live || p.dim < DP || p.rows <= 8;
+        with_padding<T>(padded, [&](auto pad) {
+            const auto product = [&](float (&out)[2][4], const T* a_tile, const T* b_tile) {
+                multiply<T, STEPS, pad.value>(out, live ? p.dim : 0, [&](float (&x)[2][4], int kk) {
+                    typename M::A a;
+                    typename M::B b0, b1;
+                    M::load_a(a, a_tile + kk * KS, PITCH, lane);
+                    M::load_b_nk(b0, b1, b_tile + kk * KS, PITCH, lane);
+                    M::mma(x[0], a, b0);
+                    M::mma(x[1], a, b1);
+                });
+            };
+            product(s, tk, sq);
+            product(dp, tv, sdo);
+        });
         const bool on0 = svis[st * KT + warp * 16 + (lane >> 2)], on1 = svis[st * KT + warp * 16 + (lane >> 2) + 8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -570,31 +604,36 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
             M::from_c(pf[kk], s, kk);
             M::from_c(kf[kk], dp, kk);
         }
+        with_padding<T>(padded, [&](auto pad) {
 #pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-            accumulate<T, RS>(dq[2 * j], dq[2 * j + 1], df, [&](typename M::B& b0, typename M::B& b1, int kk) {
-                M::load_b_kn(b0, b1, tk + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-        }
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-            float x[2][4] = {}, y[2][4] = {};
-            accumulate<T, RS>(x[0], x[1], pf, [&](typename M::B& b0, typename M::B& b1, int kk) {
-                M::load_b_kn(b0, b1, sdo + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-            accumulate<T, RS>(y[0], y[1], kf, [&](typename M::B& b0, typename M::B& b1, int kk) {
-                M::load_b_kn(b0, b1, sq + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = (lane >> 2) * PITCH + j * 16 + h * 8 + (lane & 3) * 2;
-                M::store2(tv + at, on0 ? x[h][0] : 0.f, on0 ? x[h][1] : 0.f);
-                M::store2(tv + at + 8 * PITCH, on1 ? x[h][2] : 0.f, on1 ? x[h][3] : 0.f);
-                M::store2(tk + at, on0 ? y[h][0] * p.scale : 0.f, on0 ? y[h][1] * p.scale : 0.f);
-                M::store2(tk + at + 8 * PITCH, on1 ? y[h][2] * p.scale : 0.f, on1 ? y[h][3] * p.scale : 0.f);
+            for (int j = 0; j < DP / 16; ++j) {
+                if (pad.value && j * 16 >= p.dim) break;
+                accumulate<T, RS, pad.value>(dq[2 * j], dq[2 * j + 1], df, live ? RS : 0, [&](typename M::B& b0, typename M::B& b1, int kk) {
+                    M::load_b_kn(b0, b1, tk + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
             }
-        }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < DP / 16; ++j) {
+                if (pad.value && j * 16 >= p.dim) break;
+                float x[2][4] = {}, y[2][4] = {};
+                const int used = live ? (p.rows + KS - 1) / KS : 0;
+                accumulate<T, RS, pad.value>(x[0], x[1], pf, used, [&](typename M::B& b0, typename M::B& b1, int kk) {
+                    M::load_b_kn(b0, b1, sdo + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
+                accumulate<T, RS, pad.value>(y[0], y[1], kf, used, [&](typename M::B& b0, typename M::B& b1, int kk) {
+                    M::load_b_kn(b0, b1, sq + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int at = (lane >> 2) * PITCH + j * 16 + h * 8 + (lane & 3) * 2;
+                    M::store2(tv + at, on0 ? x[h][0] : 0.f, on0 ? x[h][1] : 0.f);
+                    M::store2(tv + at + 8 * PITCH, on1 ? x[h][2] : 0.f, on1 ? x[h][3] : 0.f);
+                    M::store2(tk + at, on0 ? y[h][0] * p.scale : 0.f, on0 ? y[h][1] * p.scale : 0.f);
+                    M::store2(tk + at + 8 * PITCH, on1 ? y[h][2] * p.scale : 0.f, on1 ? y[h][3] * p.scale : 0.f);
+                }
+            }
+        });
         __syncwarp();
         const int key0 = t * KT + warp * 16;
         store_key_rows<T, DP, PITCH>(tv, gv, key_row, key0, p.lk, p.dim, lane);
@@ -694,21 +733,26 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
         const T* tq = sq + st * RT * PITCH;
         const T* td = sdo + st * RT * PITCH;
         float s[RT / 8][4] = {}, dp[RT / 8][4] = {};  // [16 keys] x [RT rows]
-        const auto product = [&](float (&out)[RT / 8][4], const T* a_tile, const T* b_tile) {
-            multiply<T, STEPS>(out, [&](float (&x)[RT / 8][4], int kk) {
-                typename M::A a;
-                M::load_a(a, a_tile + kk * KS, PITCH, lane);
+        const int left = p.rows - t * RT;
+        const bool padded = p.dim < DP || left < RT;
+        with_padding<T>(padded, [&](auto pad) {
+            const auto product = [&](float (&out)[RT / 8][4], const T* a_tile, const T* b_tile) {
+                multiply<T, STEPS, pad.value>(out, p.dim, [&](float (&x)[RT / 8][4], int kk) {
+                    typename M::A a;
+                    M::load_a(a, a_tile + kk * KS, PITCH, lane);
 #pragma unroll
-                for (int j = 0; j < RT / 16; ++j) {
-                    typename M::B b0, b1;
-                    M::load_b_nk(b0, b1, b_tile + j * 16 * PITCH + kk * KS, PITCH, lane);
-                    M::mma(x[2 * j], a, b0);
-                    M::mma(x[2 * j + 1], a, b1);
-                }
-            });
-        };
-        product(s, tk, tq);
-        product(dp, tv, td);
+                    for (int j = 0; j < RT / 16; ++j) {
+                        if (pad.value && j * 16 >= left) break;
+                        typename M::B b0, b1;
+                        M::load_b_nk(b0, b1, b_tile + j * 16 * PITCH + kk * KS, PITCH, lane);
+                        M::mma(x[2 * j], a, b0);
+                        M::mma(x[2 * j + 1], a, b1);
+                    }
+                });
+            };
+            product(s, tk, tq);
+            product(dp, tv, td);
+        });
 #pragma unroll
         for (int j = 0; j < RT / 8; ++j) {
 #pragma unroll
@@ -727,15 +771,19 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
             M::from_c(pf[kk], s, kk);
             M::from_c(df[kk], dp, kk);
         }
+        with_padding<T>(padded, [&](auto pad) {
 #pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-            accumulate<T, RS>(dv[2 * j], dv[2 * j + 1], pf, [&](typename M::B& b0, typename M::B& b1, int kk) {
-                M::load_b_kn(b0, b1, td + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-            accumulate<T, RS>(dk[2 * j], dk[2 * j + 1], df, [&](typename M::B& b0, typename M::B& b1, int kk) {
-                M::load_b_kn(b0, b1, tq + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-        }
+            for (int j = 0; j < DP / 16; ++j) {
+                if (pad.value && j * 16 >= p.dim) break;
+                const int used = (left + KS - 1) / KS;
+                accumulate<T, RS, pad.value>(dv[2 * j], dv[2 * j + 1], pf, used, [&](typename M::B& b0, typename M::B& b1, int kk) {
+                    M::load_b_kn(b0, b1, td + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
+                accumulate<T, RS, pad.value>(dk[2 * j], dk[2 * j + 1], df, used, [&](typename M::B& b0, typename M::B& b1, int kk) {
+                    M::load_b_kn(b0, b1, tq + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
+            }
+        });
     }
     copy_wait<0>();
     __syncthreads();
@@ -836,21 +884,26 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
         const T* tk = sk + st * KT * PITCH;
         const T* tv = sv + st * KT * PITCH;
         float s[KT / 8][4] = {}, dp[KT / 8][4] = {};  // [16 rows] x [KT keys]
-        const auto product = [&](float (&out)[KT / 8][4], const T* a_tile, const T* b_tile) {
-            multiply<T, STEPS>(out, [&](float (&x)[KT / 8][4], int kk) {
-                typename M::A a;
-                M::load_a(a, a_tile + warp * 16 * PITCH + kk * KS, PITCH, lane);
+        const int left = n - t * KT;
+        const bool padded = p.dim < DP || left < KT;
+        with_padding<T>(padded, [&](auto pad) {
+            const auto product = [&](float (&out)[KT / 8][4], const T* a_tile, const T* b_tile) {
+                multiply<T, STEPS, pad.value>(out, p.dim, [&](float (&x)[KT / 8][4], int kk) {
+                    typename M::A a;
+                    M::load_a(a, a_tile + warp * 16 * PITCH + kk * KS, PITCH, lane);
 #pragma unroll
-                for (int j = 0; j < KT / 16; ++j) {
-                    typename M::B b0, b1;
-                    M::load_b_nk(b0, b1, b_tile + j * 16 * PITCH + kk * KS, PITCH, lane);
-                    M::mma(x[2 * j], a, b0);
-                    M::mma(x[2 * j + 1], a, b1);
-                }
-            });
-        };
-        product(s, sq, tk);
-        product(dp, sdo, tv);
+                    for (int j = 0; j < KT / 16; ++j) {
+                        if (pad.value && j * 16 >= left) break;
+                        typename M::B b0, b1;
+                        M::load_b_nk(b0, b1, b_tile + j * 16 * PITCH + kk * KS, PITCH, lane);
+                        M::mma(x[2 * j], a, b0);
+                        M::mma(x[2 * j + 1], a, b1);
+                    }
+                });
+            };
+            product(s, sq, tk);
+            product(dp, sdo, tv);
+        });
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
             const uchar2 vis = *reinterpret_cast<const uchar2*>(svis + st * KT + j * 8 + (lane & 3) * 2);
@@ -865,12 +918,15 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
         typename M::A df[KT / KS];
 #pragma unroll
         for (int kk = 0; kk < KT / KS; ++kk) M::from_c(df[kk], dp, kk);
+        with_padding<T>(padded, [&](auto pad) {
 #pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-            accumulate<T, KT / KS>(dq[2 * j], dq[2 * j + 1], df, [&](typename M::B& b0, typename M::B& b1, int kk) {
-                M::load_b_kn(b0, b1, tk + kk * KS * PITCH + j * 16, PITCH, lane);
-            });
-        }
+            for (int j = 0; j < DP / 16; ++j) {
+                if (pad.value && j * 16 >= p.dim) break;
+                accumulate<T, KT / KS, pad.value>(dq[2 * j], dq[2 * j + 1], df, (left + KS - 1) / KS, [&](typename M::B& b0, typename M::B& b1, int kk) {
+                    M::load_b_kn(b0, b1, tk + kk * KS * PITCH + j * 16, PITCH, lane);
+                });
+            }
+        });
     }
     copy_wait<0>();
     __syncthreads();
@@ -1040,8 +1096,10 @@ size_t fwd_bytes(bool f32, int dp, int rows, int keys)
     return pitch * (rows + 4 * keys);
 }
 
-// From this many rows on the gradients run on tcgen05.
-constexpr int kTcGradRows = 64;
+// Above this many rows bf16 runs on tcgen05.  Forward, 64 x 48 rows x 700 keys x 64: 42 us here, 60 us there; 64 rows x
+// 2,000 keys: 99 and 124 us; 256 tokens of 2 shared heads and more: half the time there.  Gradients, 64 x 64 rows x 2,000
+// keys: 374 and 363 us; 256 x 20 rows x 700 keys: 407 and 498 us.
+constexpr int kTcMinRows = 64;
 
 Plan make_plan(const policy_attention& a, int sms)
 {
@@ -1053,7 +1111,7 @@ Plan make_plan(const policy_attention& a, int sms)
     pl.fwd_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     if (f32) pl.fwd_keys = pl.dp == 128 ? 32 : 64;
     else pl.fwd_keys = 64;
-    pl.tc = !f32 && rows > 64 && attend_tc_takes(make_params(a));
+    pl.tc = !f32 && rows > kTcMinRows && attend_tc_takes(make_params(a));
     if (pl.tc) pl.fwd_rows = kTcRows, pl.fwd_keys = kTcKeys;
     pl.grad_warps = f32 && pl.dp == 128 ? 2 : 4;
     const int64_t q_count = a.batch * a.lq * a.heads * a.dim, k_count = a.batch * a.lk * a.kv_heads * a.dim;
@@ -1069,7 +1127,7 @@ Plan make_plan(const policy_attention& a, int sms)
         if (pl.few_splits > 1) pl.grad_bytes = align256(sizeof(float) * pl.few_splits * q_count);
     } else {
         pl.grad_bytes = align256(sizeof(float) * (q_count / a.dim));
-        pl.grad_tc = !f32 && rows > kTcGradRows && attend_grad_tc_takes(make_params(a));
+        pl.grad_tc = !f32 && rows > kTcMinRows && attend_grad_tc_takes(make_params(a));
         if (pl.grad_tc) {
             // items differ in length where lengths do: two for each SM
             pl.key_splits = choose_splits(bh * ceil_div(a.lk, grad_tc_tile(true, a.dim)), ceil_div(rows, kGradTcStream), 2 * sms, 4);
