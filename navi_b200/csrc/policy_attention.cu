@@ -176,12 +176,17 @@ struct FwdShape {
     static constexpr int ROWS = WM * 16;
     static constexpr int PITCH = DP + Mma<T>::PAD;
     static constexpr int STAGES = 2;
+    static_assert(THREADS % (DP / 4) == 0, "a thread keeps its columns");
+    // one stage does where there is one tile, and leaves room for more blocks
+    static size_t bytes(int stages)
+    {
+        const size_t stream = kQ + 2 * stages * kTile + stages * KT;
+        return stream > kMerge ? stream : kMerge;
+    }
     static constexpr size_t kTile = sizeof(T) * KT * PITCH;
     static constexpr size_t kQ = sizeof(T) * ROWS * PITCH;
     static constexpr int OPITCH = DP + 4;
-    static constexpr size_t kStream = kQ + 2 * STAGES * kTile + STAGES * KT;
     static constexpr size_t kMerge = sizeof(float) * WN * ROWS * (OPITCH + 2);
-    static constexpr size_t kBytes = kStream > kMerge ? kStream : kMerge;
 };
 
 // WM warps along the rows (16 each), WN along the keys of a tile.
@@ -195,8 +200,8 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
     extern __shared__ __align__(128) unsigned char smem[];
     T* sq = reinterpret_cast<T*>(smem);
     T* sk = sq + S::ROWS * PITCH;
-    T* sv = sk + S::STAGES * KT * PITCH;
-    uint8_t* svis = reinterpret_cast<uint8_t*>(sv + S::STAGES * KT * PITCH);
+    T* sv = sk + p.stages * KT * PITCH;
+    uint8_t* svis = reinterpret_cast<uint8_t*>(sv + p.stages * KT * PITCH);
 
     const int split = blockIdx.x % p.splits;
     const int tile = (blockIdx.x / p.splits) % p.tiles;
@@ -335,10 +340,10 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
         if ((lane & 3) == 0) sm[r] = m0, sl[r] = l0, sm[r + 8] = m1, sl[r + 8] = l1;
     }
     __syncthreads();
-    const int chunks = p.dim / 4;
-    for (int i = threadIdx.x; i < S::ROWS * chunks; i += S::THREADS) {
-        const int r = i / chunks, d = (i - r * chunks) * 4;
-        if (r0 + r >= p.rows) break;
+    constexpr int CHUNKS = DP / 4;  // a thread keeps its columns
+    for (int i = threadIdx.x; i < S::ROWS * CHUNKS; i += S::THREADS) {
+        const int r = i / CHUNKS, d = (i % CHUNKS) * 4;
+        if (r0 + r >= p.rows || d >= p.dim) break;
         float m = sm[r];
 #pragma unroll
         for (int w = 1; w < WN; ++w) m = fmaxf(m, sm[w * S::ROWS + r]);
@@ -652,10 +657,10 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
         }
     }
     __syncthreads();
-    const int chunks = p.dim / 4;
-    for (int i = threadIdx.x; i < 16 * chunks; i += S::THREADS) {
-        const int r = i / chunks, d = (i - r * chunks) * 4;
-        if (r >= p.rows) break;
+    constexpr int CHUNKS = DP / 4;
+    for (int i = threadIdx.x; i < 16 * CHUNKS; i += S::THREADS) {
+        const int r = i / CHUNKS, d = (i % CHUNKS) * 4;
+        if (r >= p.rows || d >= p.dim) break;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
@@ -940,10 +945,10 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
         }
     }
     __syncthreads();
-    const int chunks = p.dim / 4;
-    for (int i = threadIdx.x; i < ROWS * chunks; i += S::THREADS) {
-        const int r = i / chunks, d = (i - r * chunks) * 4;
-        if (r0 + r >= p.rows) break;
+    constexpr int CHUNKS = DP / 4;
+    for (int i = threadIdx.x; i < ROWS * CHUNKS; i += S::THREADS) {
+        const int r = i / CHUNKS, d = (i % CHUNKS) * 4;
+        if (r0 + r >= p.rows || d >= p.dim) break;
         const float4 x = *reinterpret_cast<const float4*>(so + r * S::OPITCH + d);
         const int64_t at = rows.index(p, r0 + r) * p.dim + d;
         if (p.splits == 1) store4(static_cast<T*>(p.dq) + at, x.x * p.scale, x.y * p.scale, x.z * p.scale, x.w * p.scale);
@@ -1169,15 +1174,16 @@ int launched(const char* what)
 }
 
 template <typename T, int DP, int WM, int WN, int KT>
-int launch_fwd(const AttnParams& p, int64_t bh, int device, cudaStream_t stream)
+int launch_fwd(AttnParams p, int64_t bh, int device, cudaStream_t stream)
 {
     using S = FwdShape<T, DP, WM, WN, KT>;
     static std::atomic<uint64_t> done{0};
-    int rc = allow_shared(attend_kernel<T, DP, WM, WN, KT>, S::kBytes, device, done);
+    int rc = allow_shared(attend_kernel<T, DP, WM, WN, KT>, S::bytes(S::STAGES), device, done);
     if (rc != POLICY_OK) return rc;
     unsigned grid = 0;
     if ((rc = launch_blocks(bh * p.tiles * p.splits, "policy_cross_attention", grid)) != POLICY_OK) return rc;
-    attend_kernel<T, DP, WM, WN, KT><<<grid, S::THREADS, S::kBytes, stream>>>(p);
+    p.stages = p.lk <= KT ? 1 : S::STAGES;
+    attend_kernel<T, DP, WM, WN, KT><<<grid, S::THREADS, S::bytes(p.stages), stream>>>(p);
     return launched("attend_kernel");
 }
 

@@ -32,6 +32,7 @@ struct AttnParams {
     int lq, lk, heads, kv_heads, group, dim, rows;
     int tiles;        // row tiles (forward, dq) or key tiles (dk, dv) of the grid
     int splits;
+    int stages;       // of key tiles in shared memory (forward)
     float scale, scale_log2;
 };
 
