@@ -118,8 +118,11 @@ __device__ __forceinline__ void with_padding(bool padded, F&& f)
     }
 }
 
+//
+// `rest`, where not null, holds what a's rounding to bf16 left off: a second product with the same b.
 template <typename T, int STEPS, bool PADDED, typename LoadB>
-__device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const typename Mma<T>::A (&a)[STEPS], int used, LoadB&& load)
+__device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const typename Mma<T>::A (&a)[STEPS], int used, LoadB&& load,
+                                           const typename Mma<T>::A* rest = nullptr)
 {
     using M = Mma<T>;
     if constexpr (M::kExact) {
@@ -141,6 +144,10 @@ __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const
             load(b0, b1, kk);
             M::mma(c0, a[kk], b0);
             M::mma(c1, a[kk], b1);
+            if (rest) {
+                M::mma(c0, rest[kk], b0);
+                M::mma(c1, rest[kk], b1);
+            }
         }
     }
 }
@@ -476,9 +483,12 @@ struct GradShape {
     static constexpr int OPITCH = DP + 4;
     static constexpr size_t kKeys = sizeof(T) * KT * PITCH;
     // all gradients, 16 rows
-    static constexpr size_t kFewStream = 4 * kKeys + sizeof(T) * (2 * 16 * PITCH + NW * 16 * TP) + 2 * KT + 16 * 3 * sizeof(float);
     static constexpr size_t kMerge = sizeof(float) * NW * 16 * OPITCH;
-    static constexpr size_t kFew = kFewStream > kMerge ? kFewStream : kMerge;
+    static constexpr size_t few_bytes(bool two)
+    {
+        const size_t stream = 4 * kKeys + sizeof(T) * (2 * 16 * PITCH + (two ? 2 : 1) * NW * 16 * TP) + 2 * KT + 16 * 3 * sizeof(float);
+        return stream > kMerge ? stream : kMerge;
+    }
     // dk and dv: RT rows stream
     static constexpr int RT = 32;
     static constexpr size_t kKeyGrad = 2 * kKeys + 4 * sizeof(T) * RT * PITCH + 6 * RT * sizeof(float) + KT;
@@ -502,8 +512,15 @@ __device__ __forceinline__ void store_key_rows(const T* tile, T* g, int64_t row_
 }
 
 // All three gradients of up to 16 rows: K and V are read once; dk and dv of a key tile are whole when it
-// has passed, dq is summed over the tiles.
-template <typename T, int DP, int NW>
+// has passed, dq is summed over the tiles.  Memory bounds it: 1,024 x 8 heads of 16 rows and 192 keys of 64 in bf16
+// take 188 us for 823 MB, 4.4 TB/s; what is left above the memory's rate is the chain scores - weights -
+// three products of a tile, which 16 resident warps do not hide.
+//
+// TWO (bf16, up to kTwoKeys keys): the weights and their gradients enter the products as two bf16 parts.  With few keys
+// the roundings do not average out, and were 1.5 times the output's own; with many the second products cost 24 %.
+constexpr int kTwoKeys = 64;
+
+template <typename T, int DP, int NW, bool TWO>
 __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnParams p)
 {
     using M = Mma<T>;
@@ -515,7 +532,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
     T* sq = sv + 2 * KT * PITCH;
     T* sdo = sq + 16 * PITCH;
     T* str = sdo + 16 * PITCH;
-    float2* sstats = reinterpret_cast<float2*>(str + NW * 16 * S::TP);
+    float2* sstats = reinterpret_cast<float2*>(str + (TWO ? 2 : 1) * NW * 16 * S::TP);
     float* sdelta = reinterpret_cast<float*>(sstats + 16);
     uint8_t* svis = reinterpret_cast<uint8_t*>(sdelta + 16);
 
@@ -597,17 +614,26 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
                 s[j][i] = on ? w : 0.f;
                 dp[j][i] = on && !single ? w * (dp[j][i] - sdelta[r]) : 0.f;
                 const int key = (lane >> 2) + (i < 2 ? 0 : 8);
-                if constexpr (sizeof(T) == 2) tr[r * S::TP + key] = __float2bfloat16_rn(dp[j][i]);
-                else tr[r * S::TP + key] = dp[j][i];
+                if constexpr (TWO) {
+                    tr[r * S::TP + key] = __float2bfloat16_rn(dp[j][i]);
+                    tr[(NW * 16 + r) * S::TP + key] = __float2bfloat16_rn(M::left_off(dp[j][i]));
+                } else {
+                    tr[r * S::TP + key] = dp[j][i];
+                }
             }
         }
         __syncwarp();
-        typename M::A df[RS], pf[RS], kf[RS];
+        typename M::A df[RS], pf[RS], kf[RS], dr[RS], pr[RS], kr[RS];
 #pragma unroll
         for (int kk = 0; kk < RS; ++kk) {
             M::load_a(df[kk], tr + kk * KS, S::TP, lane);
             M::from_c(pf[kk], s, kk);
             M::from_c(kf[kk], dp, kk);
+            if constexpr (TWO) {
+                M::load_a(dr[kk], tr + NW * 16 * S::TP + kk * KS, S::TP, lane);
+                M::rest_of_c(pr[kk], s, kk);
+                M::rest_of_c(kr[kk], dp, kk);
+            }
         }
         with_padding<T>(padded, [&](auto pad) {
 #pragma unroll
@@ -615,7 +641,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
                 if (pad.value && j * 16 >= p.dim) break;
                 accumulate<T, RS, pad.value>(dq[2 * j], dq[2 * j + 1], df, live ? RS : 0, [&](typename M::B& b0, typename M::B& b1, int kk) {
                     M::load_b_kn(b0, b1, tk + kk * KS * PITCH + j * 16, PITCH, lane);
-                });
+                }, TWO ? dr : nullptr);
             }
             __syncwarp();
 #pragma unroll
@@ -625,10 +651,10 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
                 const int used = live ? (p.rows + KS - 1) / KS : 0;
                 accumulate<T, RS, pad.value>(x[0], x[1], pf, used, [&](typename M::B& b0, typename M::B& b1, int kk) {
                     M::load_b_kn(b0, b1, sdo + kk * KS * PITCH + j * 16, PITCH, lane);
-                });
+                }, TWO ? pr : nullptr);
                 accumulate<T, RS, pad.value>(y[0], y[1], kf, used, [&](typename M::B& b0, typename M::B& b1, int kk) {
                     M::load_b_kn(b0, b1, sq + kk * KS * PITCH + j * 16, PITCH, lane);
-                });
+                }, TWO ? kr : nullptr);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int at = (lane >> 2) * PITCH + j * 16 + h * 8 + (lane & 3) * 2;
@@ -1253,15 +1279,20 @@ template <typename T, int DP, int NW>
 int run_backward_dim(const policy_attention& a, const Plan& pl, int sms, cudaStream_t stream)
 {
     using S = GradShape<T, DP, NW>;
-    static std::atomic<uint64_t> done_few{0}, done_keys{0}, done_queries{0};
+    static std::atomic<uint64_t> done_few{0}, done_two{0}, done_keys{0}, done_queries{0};
     AttnParams p = make_params(a);
     const int64_t bh = a.batch * a.kv_heads;
     int rc = POLICY_OK;
     if (pl.few) {
         p.splits = pl.few_splits;
         p.part = static_cast<float*>(a.workspace);
-        rc = launch_grad<T>(attend_grad_few_kernel<T, DP, NW>, S::kFew, done_few, p, bh * p.splits, S::THREADS, a.device, stream,
-                            "attend_grad_few_kernel");
+        constexpr bool kTwo = sizeof(T) == 2;
+        if (kTwo && p.lk <= kTwoKeys)
+            rc = launch_grad<T>(attend_grad_few_kernel<T, DP, NW, kTwo>, S::few_bytes(kTwo), done_two, p, bh * p.splits, S::THREADS, a.device,
+                                stream, "attend_grad_few_kernel");
+        else
+            rc = launch_grad<T>(attend_grad_few_kernel<T, DP, NW, false>, S::few_bytes(false), done_few, p, bh * p.splits, S::THREADS, a.device,
+                                stream, "attend_grad_few_kernel");
         if (rc == POLICY_OK && p.splits > 1) rc = add_parts<T>(p.part, p.q_count, p.splits, p.q_count, p.dq, stream);
         return rc;
     }

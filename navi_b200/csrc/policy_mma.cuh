@@ -86,6 +86,16 @@ struct Mma<bf16> {
         a.r[2] = pack(c[2 * step + 1][0], c[2 * step + 1][1]);
         a.r[3] = pack(c[2 * step + 1][2], c[2 * step + 1][3]);
     }
+    // what that rounding leaves off, again as an A: both products together have the weights to 2^-17
+    template <int N>
+    static __device__ __forceinline__ void rest_of_c(A& a, const float (&c)[N][4], int step)
+    {
+        a.r[0] = pack(left_off(c[2 * step][0]), left_off(c[2 * step][1]));
+        a.r[1] = pack(left_off(c[2 * step][2]), left_off(c[2 * step][3]));
+        a.r[2] = pack(left_off(c[2 * step + 1][0]), left_off(c[2 * step + 1][1]));
+        a.r[3] = pack(left_off(c[2 * step + 1][2]), left_off(c[2 * step + 1][3]));
+    }
+    static __device__ __forceinline__ float left_off(float x) { return x - __bfloat162float(__float2bfloat16_rn(x)); }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi)
     {
         const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
