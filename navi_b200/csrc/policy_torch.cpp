@@ -182,7 +182,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
         REQUIRE(lengths->device() == q.device(), "key_lengths must be on the device of q");
         REQUIRE(lengths->scalar_type() == at::kInt && lengths->dim() == 1 && lengths->size(0) == b,
                 "key_lengths must be an int32 tensor of shape [batch]");
-        key_lengths = lengths->contiguous();
+        key_lengths = lengths->is_contiguous() ? *lengths : lengths->contiguous();
     }
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
         return CrossAttention::apply(q, k, v, optional(key_mask), optional(key_lengths), scale);
@@ -272,9 +272,10 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
     }
 };
 
+// (a conversion that changes nothing still costs a dispatch, a good part of a small call)
 Tensor aligned(const Tensor& t)
 {
-    const Tensor c = t.contiguous();
+    const Tensor c = t.is_contiguous() ? t : t.contiguous();
     return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
@@ -284,7 +285,7 @@ Tensor check_weight(const char* name, const OptionalTensor& w, const Tensor& x)
     REQUIRE(w->device() == x.device() && (w->scalar_type() == at::kFloat || w->scalar_type() == x.scalar_type()) && w->dim() == 1 &&
                 w->size(0) == x.size(3),
             name, " must be a [dim] tensor in float32 or the type of q, on its device");
-    return aligned(w->to(at::kFloat));
+    return aligned(w->scalar_type() == at::kFloat ? *w : w->to(at::kFloat));
 }
 
 Tensor check_table(const char* name, const OptionalTensor& table, const Tensor& x, bool positions)
@@ -295,7 +296,7 @@ Tensor check_table(const char* name, const OptionalTensor& table, const Tensor& 
     REQUIRE(table->size(2) % 8 == 0 && table->size(2) > 0 && 2 * table->size(2) <= x.size(3), name,
             ": rotary_dim must be a multiple of 16 from 16 to dim");
     REQUIRE(positions || table->size(0) >= x.size(1), name, " must have a row for every token");
-    return aligned(table->detach());
+    return aligned(table->requires_grad() ? table->detach() : *table);
 }
 
 Tensor check_positions(const char* name, const OptionalTensor& p, const Tensor& x)
@@ -303,7 +304,7 @@ Tensor check_positions(const char* name, const OptionalTensor& p, const Tensor& 
     if (!p) return Tensor();
     REQUIRE(p->device() == x.device() && p->scalar_type() == at::kInt && p->dim() == 2 && p->size(0) == x.size(0) && p->size(1) == x.size(1),
             name, " must be an int32 tensor of shape [batch, tokens] on the device of q");
-    return p->contiguous();
+    return p->is_contiguous() ? *p : p->contiguous();
 }
 
 std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptionalTensor& q_weight_, const OptionalTensor& k_weight_,
