@@ -13,7 +13,8 @@
 // All tiles come by TMA, a row tile as 64 / group tokens x group heads.  One warp follows the copies of Y: for dq
 // it zeroes K's invisible rows (0 x NaN would be NaN) and says which keys are visible, for dk and dv it brings the
 // rows' statistics.  (S may be reading a row of K while it is zeroed: that column of S is not used.)  Bound by the products: at 64 columns the two SS products read shared memory faster than its
-// 128 bytes a clock (48 clocks per 16 deep instead of 32).
+// 128 bytes a clock (48 clocks per 16 deep instead of 32).  Measured, 8 x 4,096 rows x 768 keys x 64, 8 / 4 heads: dk and dv
+// 195 us, dq 177 us, 410 us with D (314 TFLOP/s); the chain products - weights - products of a tile is what is left.
 #include <atomic>
 #include <limits>
 

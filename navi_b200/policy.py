@@ -49,7 +49,8 @@ def cross_attention(
     such as the valid rays of an observation; ``key_lengths`` [batch] (int32) makes the keys
     from that index on invisible.  What invisible keys hold (NaN and infinities included) reaches
     no output, and their gradients are 0.  A query with no visible key gives 0 and receives
-    gradient 0.  ``scale`` defaults to 1 / sqrt(dim).
+    gradient 0.  A visible value that is not finite makes what it reaches not finite.  ``scale`` defaults
+    to 1 / sqrt(dim).
 
     Returns [batch, lq, heads, dim], contiguous; differentiable once in q, k and v.  Scores,
     softmax and sums are held in 32 bits; with bfloat16 the softmax weights enter the product with
