@@ -118,7 +118,7 @@ __device__ __forceinline__ void with_padding(bool padded, F&& f)
     }
 }
 
-//
+// c0 and c1 += a with the two B tiles that load(b0, b1, kk) brings.  f32 adds the steps up apart first.
 // `rest`, where not null, holds what a's rounding to bf16 left off: a second product with the same b.
 template <typename T, int STEPS, bool PADDED, typename LoadB>
 __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const typename Mma<T>::A (&a)[STEPS], int used, LoadB&& load,
@@ -199,7 +199,13 @@ struct FwdShape {
 // WM warps along the rows (16 each), WN along the keys of a tile.  With few rows memory bounds it: one query with 4
 // heads to a key head over 64 x 12,288 keys of 64 in bf16 takes 72 us for 404 MB, 5.6 TB/s; in f32 195 us, bound by the
 // three TF32 products and the splitting of every operand (35 TFLOP/s where rows are many).
-template <typename T, int DP, int WM, int WN, int KT>
+//
+// TWO (bf16, up to kTwoKeysFwd keys): the weights enter the product with v as two bf16 parts, since the gradients take
+// do . out from it, where a weight's rounding does not cancel against the exact one beside it; with many keys the
+// roundings average out, and the second product costs 13 % at 64 keys and 37 % where rows and keys are many.
+constexpr int kTwoKeysFwd = 16;
+
+template <typename T, int DP, int WM, int WN, int KT, bool TWO>
 __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p)
 {
     using M = Mma<T>;
@@ -315,6 +321,11 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
         typename M::A pf[KSL / KS];
 #pragma unroll
         for (int kk = 0; kk < KSL / KS; ++kk) M::from_c(pf[kk], s, kk);
+        typename M::A pr[TWO ? KSL / KS : 1];
+        if constexpr (TWO) {
+#pragma unroll
+            for (int kk = 0; kk < KSL / KS; ++kk) M::rest_of_c(pr[kk], s, kk);
+        }
         with_padding<T>(padded, [&](auto pad) {
 #pragma unroll
             for (int j = 0; j < DP / 16; ++j) {
@@ -326,7 +337,7 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
                 }
                 accumulate<T, KSL / KS, pad.value>(o[2 * j], o[2 * j + 1], pf, (left + KS - 1) / KS, [&](typename M::B& b0_, typename M::B& b1_, int kk) {
                     M::load_b_kn(b0_, b1_, tv + kk * KS * PITCH + j * 16, PITCH, lane);
-                });
+                }, TWO ? pr : nullptr);
             }
         });
     }
@@ -1201,18 +1212,26 @@ int launched(const char* what)
     return e == cudaSuccess ? POLICY_OK : cuda_fail(e, what);
 }
 
-template <typename T, int DP, int WM, int WN, int KT>
-int launch_fwd(AttnParams p, int64_t bh, int device, cudaStream_t stream)
+template <typename T, int DP, int WM, int WN, int KT, bool TWO>
+int launch_fwd_tile(AttnParams p, int64_t bh, int device, cudaStream_t stream)
 {
     using S = FwdShape<T, DP, WM, WN, KT>;
     static std::atomic<uint64_t> done{0};
-    int rc = allow_shared(attend_kernel<T, DP, WM, WN, KT>, S::bytes(S::STAGES), device, done);
+    int rc = allow_shared(attend_kernel<T, DP, WM, WN, KT, TWO>, S::bytes(S::STAGES), device, done);
     if (rc != POLICY_OK) return rc;
     unsigned grid = 0;
     if ((rc = launch_blocks(bh * p.tiles * p.splits, "policy_cross_attention", grid)) != POLICY_OK) return rc;
     p.stages = p.lk <= KT ? 1 : S::STAGES;
-    attend_kernel<T, DP, WM, WN, KT><<<grid, S::THREADS, S::bytes(p.stages), stream>>>(p);
+    attend_kernel<T, DP, WM, WN, KT, TWO><<<grid, S::THREADS, S::bytes(p.stages), stream>>>(p);
     return launched("attend_kernel");
+}
+
+template <typename T, int DP, int WM, int WN, int KT>
+int launch_fwd(const AttnParams& p, int64_t bh, int device, cudaStream_t stream)
+{
+    constexpr bool kTwo = sizeof(T) == 2;
+    if (kTwo && p.lk <= kTwoKeysFwd) return launch_fwd_tile<T, DP, WM, WN, KT, kTwo>(p, bh, device, stream);
+    return launch_fwd_tile<T, DP, WM, WN, KT, false>(p, bh, device, stream);
 }
 
 template <typename T, int DP>
