@@ -1229,8 +1229,10 @@ int launch_fwd_tile(AttnParams p, int64_t bh, int device, cudaStream_t stream)
 template <typename T, int DP, int WM, int WN, int KT>
 int launch_fwd(const AttnParams& p, int64_t bh, int device, cudaStream_t stream)
 {
-    constexpr bool kTwo = sizeof(T) == 2;
-    if (kTwo && p.lk <= kTwoKeysFwd) return launch_fwd_tile<T, DP, WM, WN, KT, kTwo>(p, bh, device, stream);
+    if constexpr (sizeof(T) == 2) {
+        constexpr int kFew = WM * 32 / (DP / 8) > kTwoKeysFwd ? 2 * kTwoKeysFwd : kTwoKeysFwd;  // a thread loads a key at least
+        if (p.lk <= kTwoKeysFwd) return launch_fwd_tile<T, DP, WM, 1, kFew, true>(p, bh, device, stream);
+    }
     return launch_fwd_tile<T, DP, WM, WN, KT, false>(p, bh, device, stream);
 }
 
