@@ -200,10 +200,10 @@ struct FwdShape {
 // heads to a key head over 64 x 12,288 keys of 64 in bf16 takes 72 us for 404 MB, 5.6 TB/s; in f32 195 us, bound by the
 // three TF32 products and the splitting of every operand (35 TFLOP/s where rows are many).
 //
-// TWO (bf16, up to kTwoKeysFwd keys): the weights enter the product with v as two bf16 parts, since the gradients take
+// TWO (bf16, up to kFewKeysFwd keys): the weights enter the product with v as two bf16 parts, since the gradients take
 // do . out from it, where a weight's rounding does not cancel against the exact one beside it; with many keys the
 // roundings average out, and the second product costs 13 % at 64 keys and 37 % where rows and keys are many.
-constexpr int kTwoKeysFwd = 16;
+constexpr int kFewKeysFwd = 32;
 
 template <typename T, int DP, int WM, int WN, int KT, bool TWO>
 __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p)
@@ -1226,13 +1226,19 @@ int launch_fwd_tile(AttnParams p, int64_t bh, int device, cudaStream_t stream)
     return launched("attend_kernel");
 }
 
+// Up to 16 and up to 32 keys have tiles of their own, with all warps along the rows: a tile of 64 computes and joins
+// keys that are not there, and its shared memory keeps blocks away.  1,024 x 8 heads of 16 rows of 64, in bf16 with 16
+// keys 50 us with the larger tile and 25 here, with 24 keys 52 and 31; in f32 92 and 43, 105 and 62; 32 rows and 32 keys
+// of 64 in bf16 75 and 54, in f32 144 and 97; 8,132 x 4 rows and 3 keys of 64 in f32 18.8 and 16.5.  f32 tiles of dim 128
+// hold 32 keys as they are.
 template <typename T, int DP, int WM, int WN, int KT>
 int launch_fwd(const AttnParams& p, int64_t bh, int device, cudaStream_t stream)
 {
-    if constexpr (sizeof(T) == 2) {
-        constexpr int kFew = WM * 32 / (DP / 8) > kTwoKeysFwd ? 2 * kTwoKeysFwd : kTwoKeysFwd;  // a thread loads a key at least
-        if (p.lk <= kTwoKeysFwd) return launch_fwd_tile<T, DP, WM, 1, kFew, true>(p, bh, device, stream);
-    }
+    constexpr bool kTwo = sizeof(T) == 2;
+    constexpr int kLeast = WM * 32 / (DP / Mma<T>::VEC) > 16 ? 32 : 16;  // a thread loads a key at least
+    if (p.lk <= 16) return launch_fwd_tile<T, DP, WM, 1, kLeast, kTwo>(p, bh, device, stream);
+    if constexpr (KT > kFewKeysFwd)
+        if (p.lk <= kFewKeysFwd) return launch_fwd_tile<T, DP, WM, 1, kFewKeysFwd, kTwo>(p, bh, device, stream);
     return launch_fwd_tile<T, DP, WM, WN, KT, false>(p, bh, device, stream);
 }
 

@@ -94,6 +94,18 @@ def test_what_invisible_keys_hold_does_not_matter(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mask", ["none", "both"])
+@pytest.mark.parametrize("dim", [24, 64, 96])
+@pytest.mark.parametrize("lk", [1, 2, 15, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("lq", [1, 13, 30])  # 2, 26 and 60 rows to a key head: the three row tiles
+def test_short_key_lists(lq, lk, dim, mask, dtype):
+    q, k, v, do, kw, visible = inputs((3, lq, lk, 4, 2, dim), dtype, seed=lk, mask=mask, poison=True)
+    out = policy.cross_attention(q, k, v, **kw)
+    want = ref.attention_gradients(q, k, v, do, visible)[0]
+    ref.assert_close(out, want, ref.FORWARD[dtype], "out")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lq", [1, 16, 17, 100])
 def test_no_visible_key(lq, dtype):
     q, k, v, do, _, _ = inputs((2, lq, 70, 4, 2, 64), dtype)
