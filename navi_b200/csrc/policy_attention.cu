@@ -118,7 +118,11 @@ __device__ __forceinline__ void with_padding(bool padded, F&& f)
     }
 }
 
-// c0 and c1 += a with the two B tiles that load(b0, b1, kk) brings.  f32 adds the steps up apart first.
+// f32 adds up this many k steps apart before it adds them, rounded to nearest, to the sum.
+constexpr int kFlush = 4;
+
+// c0 and c1 += a with the two B tiles that load(b0, b1, kk) brings, in f32 kFlush steps apart: with the 8 of a 64-key tile in
+// one chain, out was off by 2^-20 of its size where values have one sign.
 // `rest`, where not null, holds what a's rounding to bf16 left off: a second product with the same b.
 template <typename T, int STEPS, bool PADDED, typename LoadB>
 __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const typename Mma<T>::A (&a)[STEPS], int used, LoadB&& load,
@@ -126,17 +130,21 @@ __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const
 {
     using M = Mma<T>;
     if constexpr (M::kExact) {
-        float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < STEPS; ++kk) {
-            if (PADDED && kk >= used) break;
-            typename M::B b0, b1;
-            load(b0, b1, kk);
-            M::mma(t0, a[kk], b0);
-            M::mma(t1, a[kk], b1);
+        for (int k0 = 0; k0 < STEPS; k0 += kFlush) {
+            if (PADDED && k0 >= used) break;
+            float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = k0; kk < k0 + kFlush && kk < STEPS; ++kk) {
+                if (PADDED && kk >= used) break;
+                typename M::B b0, b1;
+                load(b0, b1, kk);
+                M::mma(t0, a[kk], b0);
+                M::mma(t1, a[kk], b1);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c0[i] += t0[i], c1[i] += t1[i];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c0[i] += t0[i], c1[i] += t1[i];
     } else {
 #pragma unroll
         for (int kk = 0; kk < STEPS; ++kk) {
@@ -153,9 +161,7 @@ __device__ __forceinline__ void accumulate(float (&c0)[4], float (&c1)[4], const
 }
 
 // The products of a 16-row A with N pairs of B tiles, k step by k step: c (+)= a b.  f32 adds up kFlush steps apart
-// and then rounds to nearest, for the same reason.
-constexpr int kFlush = 4;
-
+// here too.
 template <typename T, int STEPS, bool PADDED, int N, typename Step>
 __device__ __forceinline__ void multiply(float (&c)[N][4], int dim, Step&& step)
 {
