@@ -321,12 +321,18 @@ __global__ void __launch_bounds__(WM * WN * 32) attend_kernel(const AttnParams p
             s[j][1] = exp2_fast(fmaf(s[j][1], c, -b0));
             s[j][2] = exp2_fast(fmaf(s[j][2], c, -b1));
             s[j][3] = exp2_fast(fmaf(s[j][3], c, -b1));
-            l0 += s[j][0] + s[j][1];
-            l1 += s[j][2] + s[j][3];
         }
         typename M::A pf[KSL / KS];
 #pragma unroll
-        for (int kk = 0; kk < KSL / KS; ++kk) M::from_c(pf[kk], s, kk);
+        for (int kk = 0; kk < KSL / KS; ++kk) {
+            M::from_c(pf[kk], s, kk);
+            if constexpr (!TWO) M::to_c(s, pf[kk], kk);
+        }
+#pragma unroll
+        for (int j = 0; j < KSL / 8; ++j) {
+            l0 += s[j][0] + s[j][1];
+            l1 += s[j][2] + s[j][3];
+        }
         typename M::A pr[TWO ? KSL / KS : 1];
         if constexpr (TWO) {
 #pragma unroll

@@ -86,6 +86,18 @@ struct Mma<bf16> {
         a.r[2] = pack(c[2 * step + 1][0], c[2 * step + 1][1]);
         a.r[3] = pack(c[2 * step + 1][2], c[2 * step + 1][3]);
     }
+    // The rounded weights back, for the sum that divides them: so they add up to 1, and what their roundings leave is off by
+    // the spread of the values, not by their mean (which do . out would carry into every weight's gradient: rows of dq
+    // off by more than their own size).
+    template <int N>
+    static __device__ __forceinline__ void to_c(float (&c)[N][4], const A& a, int step)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float* at = c[2 * step + (i >> 1)] + 2 * (i & 1);
+            at[0] = __uint_as_float(a.r[i] << 16), at[1] = __uint_as_float(a.r[i] & 0xffff0000u);
+        }
+    }
     // what that rounding leaves off, again as an A: both products together have the weights to 2^-17
     template <int N>
     static __device__ __forceinline__ void rest_of_c(A& a, const float (&c)[N][4], int step)
@@ -166,6 +178,8 @@ struct Mma<float> {
     {
         a.r[0] = c[step][0], a.r[1] = c[step][2], a.r[2] = c[step][1], a.r[3] = c[step][3];
     }
+    template <int N>
+    static __device__ __forceinline__ void to_c(float (&)[N][4], const A&, int) {}
     static __device__ __forceinline__ void store2(float* p, float a, float b)
     {
         *reinterpret_cast<float2*>(p) = make_float2(a, b);

@@ -31,7 +31,7 @@ from tests import policy_ref as ref
 pytestmark = pytest.mark.gpu
 
 DEV = torch.device("cuda", 0)
-DTYPES = [torch.float32]
+DTYPES = [torch.float32, torch.bfloat16]
 
 
 def bounds(q, k, v, do, visible):
