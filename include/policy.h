@@ -147,8 +147,9 @@ POLICY_API int policy_qk_norm_rotary_backward(const policy_qk_norm* args, void* 
  *   out = c * grad  (out may be grad itself).
  * The norm is summed in 32 bits per thread and 64 bits across threads, in an order that
  * depends on the sizes and alignments alone.  A norm that is not finite scales by what
- * the formula gives (an infinite norm by 0, NaN by NaN).  norm receives one f32.  grad and
- * out must not overlap unless they are the same address. */
+ * the formula gives (an infinite norm by 0, NaN by NaN).  norm receives one f32.  No two
+ * outputs overlap, and an output overlaps no gradient but its own, which is then at the
+ * same address: POLICY_ERR_INVALID otherwise. */
 typedef struct policy_grad {
     const void* grad;
     void* out;

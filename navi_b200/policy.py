@@ -115,8 +115,9 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float, *,
     """The 2-norm over all values of ``grads``, and every gradient times min(1, max_norm / (norm + 1e-6)).
 
     The gradients are changed in place, or written to ``out`` (tensors of the same shapes, types and
-    strides).  They are float32 or bfloat16, in any mixture, dense in memory, all on one device, and no two share
-    memory.  Returns the norm before clipping, a float32 tensor without axes on the device: nothing waits for it.
+    strides).  They are float32 or bfloat16, in any mixture, dense in memory, all on one device.  What is written shares
+    memory with nothing else: no two of the changed gradients, and no ``out`` with a gradient other than its
+    own.  Returns the norm before clipping, a float32 tensor without axes on the device: nothing waits for it.
     The sums do not depend on timing.  A norm that is not finite scales as the formula says: an infinite one
     by 0, NaN by NaN.
     """
