@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -26,6 +27,12 @@ using OptionalTensor = std::optional<Tensor>;
 bool known_type(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
 int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? POLICY_F32 : POLICY_BF16; }
 
+// A result without a tangent would say that the derivative is 0.
+void check_tangent(const char* name, const Tensor& t)
+{
+    REQUIRE(!t._fw_grad(0).defined(), name, " carries a tangent: forward-mode derivatives are not supported");
+}
+
 void check_heads(const char* name, const Tensor& t, const Tensor& like)
 {
     REQUIRE(t.is_cuda(), name, " must be a CUDA tensor. CPU tensors are not supported.");
@@ -33,6 +40,7 @@ void check_heads(const char* name, const Tensor& t, const Tensor& like)
     REQUIRE(known_type(t), name, " must be float32 or bfloat16");
     REQUIRE(t.scalar_type() == like.scalar_type(), name, " must have the type of q");
     REQUIRE(t.device() == like.device(), name, " must be on the device of q");
+    check_tangent(name, t);
 }
 
 // The tensor, or a contiguous copy where its rows are not dense or not 16-byte aligned.
@@ -284,6 +292,7 @@ Tensor check_weight(const char* name, const OptionalTensor& w, const Tensor& x)
     REQUIRE(w->device() == x.device() && (w->scalar_type() == at::kFloat || w->scalar_type() == x.scalar_type()) && w->dim() == 1 &&
                 w->size(0) == x.size(3),
             name, " must be a [dim] tensor in float32 or the type of q, on its device");
+    check_tangent(name, *w);
     return aligned(w->scalar_type() == at::kFloat ? *w : w->to(at::kFloat));
 }
 
@@ -346,10 +355,15 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
     REQUIRE(outs.size() == grads.size(), "out must have one tensor for every gradient");
     const at::Device device = grads[0].device();
     REQUIRE(device.is_cuda(), "grads must be CUDA tensors. CPU tensors are not supported.");
+    const bool tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // asked once, not of every tensor
     std::vector<policy_grad> table(grads.size());
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor &g = grads[i], &o = outs[i];
         REQUIRE(known_type(g), "grads must be float32 or bfloat16");
+        if (tangents) {
+            check_tangent("a tensor of grads", g);
+            check_tangent("a tensor of out", o);
+        }
         REQUIRE(g.device() == device, "grads must all be on one device");
         REQUIRE(g.is_non_overlapping_and_dense(), "grads must be dense in memory");
         REQUIRE(o.is_same(g) || (o.device() == device && o.scalar_type() == g.scalar_type() && o.sizes() == g.sizes() && o.strides() == g.strides()),
