@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -26,6 +27,9 @@ using OptionalTensor = std::optional<Tensor>;
 
 bool known_type(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
 int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? POLICY_F32 : POLICY_BF16; }
+
+// A trace sees no call of this module: it would hold the result as a constant.
+void check_not_traced() { REQUIRE(!torch::jit::tracer::isTracing(), "the policy operators cannot be traced"); }
 
 // A result without a tangent would say that the derivative is 0.
 void check_tangent(const char* name, const Tensor& t)
@@ -168,6 +172,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptionalTensor& mask, const OptionalTensor& lengths,
                        const std::optional<double>& scale_)
 {
+    check_not_traced();
     check_heads("q", q, q);
     check_heads("k", k, q);
     check_heads("v", v, q);
@@ -319,6 +324,7 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, cons
                                           const OptionalTensor& q_table_, const OptionalTensor& k_table_,
                                           const OptionalTensor& q_positions_, const OptionalTensor& k_positions_, double eps)
 {
+    check_not_traced();
     check_heads("q", q, q);
     check_heads("k", k, q);
     const int64_t d = q.size(3);
@@ -349,6 +355,7 @@ std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, cons
 
 Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const std::optional<std::vector<Tensor>>& out)
 {
+    check_not_traced();
     REQUIRE(max_norm >= 0.0, "max_norm must not be negative");
     REQUIRE(!grads.empty(), "grads must not be empty");
     const std::vector<Tensor>& outs = out ? *out : grads;

@@ -10,7 +10,7 @@ The tensors are float32 or bfloat16 on a B200.  Every call is asynchronous on th
 current CUDA stream and never synchronises the host; its outputs and scratch come from torch's
 allocator on that stream.  There is no CPU path: a missing native library or a non-CUDA tensor raises
 RuntimeError, and so does an argument of the wrong shape or type.  Derivatives are those of reverse mode:
-a tensor that carries a forward-mode tangent raises RuntimeError.
+a tensor that carries a forward-mode tangent raises RuntimeError, and so does a call inside ``torch.jit.trace``.
 """
 
 from __future__ import annotations

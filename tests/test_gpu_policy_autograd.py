@@ -1,4 +1,4 @@
-"""What the policy operators cannot differentiate is an error, not a result without its derivative."""
+"""What the policy operators cannot differentiate or hand to a trace is an error, not a result that has lost its inputs."""
 
 from __future__ import annotations
 
@@ -50,3 +50,12 @@ def test_a_tangent_of_a_clipped_gradient_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 policy.clip_grad_norm(grads, 0.1, out=outs)
     assert torch.equal(g, before)
+
+
+def test_tracing_is_refused():
+    """A trace would keep the result of the inputs that it was made with."""
+    q, k = values(2, 3, 4, 32), values(2, 9, 2, 32)
+    for call in (lambda x: policy.cross_attention(x, k, k), lambda x: policy.qk_norm_rotary(x, k)[0], lambda x: policy.clip_grad_norm([x], 1.0)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, q)
+        call(q)
