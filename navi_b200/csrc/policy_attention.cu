@@ -566,7 +566,6 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
     const Rows rows{bh / p.kv_heads, bh % p.kv_heads, p.group};
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = visible_keys(p, rows.b);
-    const bool single = n == 1;  // the softmax of one score is constant: its gradient is 0, not a rounding of it
     const int tiles = (p.lk + KT - 1) / KT;
     const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / p.splits);
     const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / p.splits);
@@ -587,6 +586,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
             sdelta[r] = r < p.rows ? x : 0.f;
         }
     }
+    const bool lone = lone_key(p, rows.b, n);
 
     float dq[DP / 8][4];
 #pragma unroll
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_few_kernel(const AttnPara
                 const bool on = (i < 2 ? on0 : on1) && st_r.y != 0.f;
                 const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -st_r.x)) * st_r.y;
                 s[j][i] = on ? w : 0.f;
-                dp[j][i] = on && !single ? w * (dp[j][i] - sdelta[r]) : 0.f;
+                dp[j][i] = on && !lone ? w * (dp[j][i] - sdelta[r]) : 0.f;
                 const int key = (lane >> 2) + (i < 2 ? 0 : 8);
                 if constexpr (TWO) {
                     tr[r * S::TP + key] = __float2bfloat16_rn(dp[j][i]);
@@ -747,7 +747,6 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
     const Rows rows{bh / p.kv_heads, bh % p.kv_heads, p.group};
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = visible_keys(p, rows.b);
-    const bool single = n == 1;
     const int row_tiles = (p.rows + RT - 1) / RT;
     const int t0 = static_cast<int>(static_cast<int64_t>(row_tiles) * split / p.splits);
     const int t1 = static_cast<int>(static_cast<int64_t>(row_tiles) * (split + 1) / p.splits);
@@ -769,6 +768,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
     };
     if (t0 < t1) issue(t0, 0);
     copy_commit();
+    const bool lone = lone_key(p, rows.b, n);
 
     float dk[DP / 8][4], dv[DP / 8][4];
 #pragma unroll
@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_keys_kernel(const AttnPar
                 const bool on = (i < 2 ? on0 : on1) && st_r.y != 0.f;
                 const float w = exp2_fast(fmaf(s[j][i], p.scale_log2, -st_r.x)) * st_r.y;
                 s[j][i] = on ? w : 0.f;
-                dp[j][i] = on && !single ? w * (dp[j][i] - sdelta[st * RT + r]) : 0.f;
+                dp[j][i] = on && !lone ? w * (dp[j][i] - sdelta[st * RT + r]) : 0.f;
             }
         }
         typename M::A pf[RS], df[RS];
@@ -918,9 +918,10 @@ __global__ void __launch_bounds__(NW * 32) attend_grad_queries_kernel(const Attn
     for (int h = 0; h < 2; ++h) {
         const int r = r0 + warp * 16 + (lane >> 2) + 8 * h;
         const int64_t row = rows.index(p, min(r, p.rows - 1));
-        stats[h] = r < p.rows && n > 1 ? p.stats[row] : make_float2(0.f, 0.f);  // one visible key: no gradient
+        stats[h] = r < p.rows ? p.stats[row] : make_float2(0.f, 0.f);
         delta[h] = r < p.rows ? p.delta[row] : 0.f;
     }
+    if (lone_key(p, rows.b, n)) stats[0].y = stats[1].y = 0.f;  // no gradient
     float dq[DP / 8][4];
 #pragma unroll
     for (int j = 0; j < DP / 8; ++j)

@@ -67,6 +67,34 @@ __device__ __forceinline__ int visible_keys(const AttnParams& p, int64_t b)
     return min(max(__ldg(p.lengths + b), 0), p.lk);
 }
 
+// Whether at most one key of batch b is visible, n being visible_keys: the softmax of one score is constant, and its
+// gradient is 0, not a rounding of it.  For a whole warp; reads the mask up to the second visible key, as a rule in its
+// first 512 bytes.
+__device__ __forceinline__ bool lone_key(const AttnParams& p, int64_t b, int n)
+{
+    if (n <= 1 || !p.mask) return n <= 1;
+    const uint8_t* mask = p.mask + b * p.mask_stride;
+    const int lane = threadIdx.x & 31;
+    const auto ones = [](uint32_t w) { return __popc(__vsetne4(w, 0u)); };
+    int at = 0, seen = 0;
+    if (reinterpret_cast<uintptr_t>(mask) % 16 == 0) {
+        for (; at + 512 <= n && seen < 2; at += 512) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(mask + at) + lane);
+            seen += __reduce_add_sync(0xffffffffu, ones(w.x) + ones(w.y) + ones(w.z) + ones(w.w));
+        }
+    }
+    for (; at < n && seen < 2; at += 256) {
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = at + i * 32 + lane;
+            if (key < n) mine += __ldg(mask + key) != 0;
+        }
+        seen += __reduce_add_sync(0xffffffffu, mine);
+    }
+    return seen < 2;
+}
+
 __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
 // 4 values of a row

@@ -309,12 +309,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_grad_tc_kernel(const __gri
             if (kKeys) {
                 on = r < item.n;
                 if (p.mask && on) on = __ldg(p.mask + item.rows.b * p.mask_stride + r) != 0;
-            } else if (in && item.n > 1) {  // the softmax of one score is constant: its gradient is 0, not a rounding of it
+            } else if (in) {
                 const int64_t row = item.rows.index(p, r);
                 const float2 st = p.stats[row];
                 if (st.y != 0.f) exponent = st.x - log2f(st.y), delta = p.delta[row];
             }
-            const bool slope = kKeys ? on && item.n > 1 : exponent != INFINITY;
+            const bool slope = !lone_key(p, item.rows.b, item.n) && (kKeys ? on : exponent != INFINITY);
             bool ok = __all_sync(0xffffffffu, !*broken);
             for (int t = item.t0; t < item.t1 && ok; ++t, ++uses, ++tiles) {
                 const int st = uses % ST;

@@ -126,3 +126,25 @@ def test_many_keys(lq, lk, dim, peak, mean, dtype):
 def test_small_calls(shape, kind, dtype):
     for seed in range(50):
         check(shape, dtype, kind, 1.0, 0.0, seed)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lk", [5, 70, 512, 1300])  # rows of the mask that start on 16 bytes and do not
+@pytest.mark.parametrize("lq,dim", [(1, 64), (17, 64), (100, 64), (100, 128)])
+def test_one_visible_key(lq, dim, lk, dtype):
+    """The softmax of one score is constant: however the key is made the only one, dq and dk are 0 and not a rounding of it."""
+    q, k, v, do = (torch.randn(5, n, h, dim, device=DEV).to(dtype) for n, h in ((lq, 4), (lk, 2), (lk, 2), (lq, 4)))
+    where = [0, lk - 1, lk // 2, 1]
+    mask = torch.zeros(5, lk, dtype=torch.bool, device=DEV)
+    mask[range(4), where] = True
+    mask[4, [0, lk - 1]] = True
+    mask[3, 2:] = True  # beyond its length
+    lengths = torch.tensor([lk, lk, lk, 2, lk], dtype=torch.int32, device=DEV)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = policy.cross_attention(*leaves, key_mask=mask, key_lengths=lengths)
+    dq, dk, dv = torch.autograd.grad(out, leaves, do)
+    assert not dq[:4].any() and not dk[:4].any()
+    for b, j in enumerate(where):
+        ref.assert_close(out[b], v.detach()[b, j].double().repeat_interleave(2, 0).expand_as(out[b]), ref.ONE_ROUNDING[dtype], "out")
+        ref.assert_close(dv[b, j], do[b].double().reshape(lq, 2, 2, dim).sum((0, 2)), 2 * ref.ONE_ROUNDING[dtype], "dv")
+    assert (dq[4] != 0).double().mean() > 0.9 and (dk[4, [0, lk - 1]] != 0).double().mean() > 0.9  # two visible keys
