@@ -34,7 +34,8 @@ typedef enum policy_status {
     POLICY_OK = 0,
     POLICY_ERR_INVALID = -1,     /* bad argument (null pointer, size, alignment, range) */
     POLICY_ERR_CUDA = -3,        /* a CUDA runtime call failed */
-    POLICY_ERR_UNSUPPORTED = -5  /* device is not sm_100 */
+    POLICY_ERR_UNSUPPORTED = -5, /* device is not sm_100 */
+    POLICY_ERR_STALLED = -6      /* a wait inside an earlier attention kernel ran out: its rows are NaN */
 } policy_status;
 
 typedef enum policy_dtype {
@@ -90,6 +91,13 @@ typedef struct policy_attention {
     void* dv;
     void* workspace;
 } policy_attention;
+
+/* A wait inside a kernel is bounded.  One that runs out, which only a defect could cause, leaves NaN in
+ * the rows that it belongs to and sets this word, in pinned host memory that every device sees, to 1.  The next
+ * call of policy_cross_attention or policy_cross_attention_backward clears it and returns
+ * POLICY_ERR_STALLED; a caller that has synchronised with its last call may read it.  Null without a
+ * CUDA device. */
+POLICY_API volatile int32_t* policy_stall_word(void);
 
 POLICY_API uint64_t policy_cross_attention_workspace_bytes(const policy_attention* args, int backward);
 POLICY_API int policy_cross_attention(const policy_attention* args, void* stream);

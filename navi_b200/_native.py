@@ -224,6 +224,7 @@ POLICY_BF16 = 1
 POLICY_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "policy_version": (c_int, []),
     "policy_last_error": (c_char_p, []),
+    "policy_stall_word": (c_void_p, []),
     "policy_cross_attention_workspace_bytes": (c_uint64, [c_void_p, c_int]),
     "policy_cross_attention": (c_int, [c_void_p, c_void_p]),
     "policy_cross_attention_backward": (c_int, [c_void_p, c_void_p]),

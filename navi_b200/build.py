@@ -168,11 +168,11 @@ def build_policy_torch(force: bool = False) -> Path:
 
 
 def build_probe(force: bool = False) -> Path:
-    """libnavi_probe.so: the L2 read-bandwidth probe bench.py reports the L2 roofline against,
-    and the check of the trace kernel's exit quotient against the IEEE division."""
+    """libnavi_probe.so: the L2 read-bandwidth probe bench.py reports the L2 roofline against, and checks of device
+    functions: the trace kernel's exit quotient against the IEEE division, the policy kernels' bounded wait."""
     out = LIB / "libnavi_probe.so"
-    srcs = [CSRC / "peak_probe.cu", CSRC / "quotient_check.cu"]
-    if force or _stale(out, srcs + [CSRC / "exit_quotient.cuh"]):
+    srcs = [CSRC / "peak_probe.cu", CSRC / "quotient_check.cu", CSRC / "wait_check.cu"]
+    if force or _stale(out, srcs + [CSRC / "exit_quotient.cuh", CSRC / "policy_tcgen05.cuh"]):
         LIB.mkdir(parents=True, exist_ok=True)
         tmp = out.with_suffix(".so.tmp")
         _run([_nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",

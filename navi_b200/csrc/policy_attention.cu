@@ -1271,6 +1271,12 @@ int launch_fwd_rows(const AttnParams& p, const Plan& pl, int64_t bh, int device,
     }
 }
 
+int set_stall_word(AttnParams& p)
+{
+    p.stalled = stall_word();
+    return p.stalled ? POLICY_OK : fail(POLICY_ERR_CUDA, "cudaHostAlloc failed");
+}
+
 template <typename T>
 int run_forward(const policy_attention& a, const Plan& pl, int sms, cudaStream_t stream)
 {
@@ -1282,7 +1288,9 @@ int run_forward(const policy_attention& a, const Plan& pl, int sms, cudaStream_t
         p.part = static_cast<float*>(a.workspace);
         p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + align256(sizeof(float) * p.splits * p.q_count));
     }
-    int rc = pl.tc         ? launch_attend_tc(p, bh, sms, a.device, stream)
+    int rc = pl.tc ? set_stall_word(p) : POLICY_OK;
+    if (rc != POLICY_OK) return rc;
+    rc = pl.tc         ? launch_attend_tc(p, bh, sms, a.device, stream)
              : pl.dp == 32 ? launch_fwd_rows<T, 32>(p, pl, bh, a.device, stream)
              : pl.dp == 64 ? launch_fwd_rows<T, 64>(p, pl, bh, a.device, stream)
                            : launch_fwd_rows<T, 128>(p, pl, bh, a.device, stream);
@@ -1346,6 +1354,7 @@ int run_backward_dim(const policy_attention& a, const Plan& pl, int sms, cudaStr
     attend_delta_kernel<T><<<grid, 256, 0, stream>>>(p, delta);
     if ((rc = launched("attend_delta_kernel")) != POLICY_OK) return rc;
     p.delta = delta;
+    if (pl.grad_tc && (rc = set_stall_word(p)) != POLICY_OK) return rc;
 
     p.splits = pl.key_splits;
     p.tiles = ceil_div(p.lk, pl.grad_tc ? grad_tc_tile(true, p.dim) : S::KT);
@@ -1416,6 +1425,8 @@ int entry(const policy_attention* a, bool is_backward, F&& run)
     if (rc != POLICY_OK) return rc;
     const DeviceInfo info = device_info(a->device);
     if (info.status != POLICY_OK) return info.status;
+    const int stalled = check_stall();
+    if (stalled != POLICY_OK) return stalled;
     DeviceScope scope(a->device);
     if (scope.error() != cudaSuccess) return cuda_fail(scope.error(), "cudaSetDevice");
     return run(info.sms);

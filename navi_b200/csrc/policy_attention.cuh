@@ -34,6 +34,7 @@ struct AttnParams {
     int splits;
     int stages;       // of key tiles in shared memory (forward)
     float scale, scale_log2;
+    int32_t* stalled;  // tcgen05: the host's word for a wait that ran out
 };
 
 __device__ __forceinline__ float exp2_fast(float x)

@@ -415,6 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_grad_tc_kernel(const __gri
     if (warp == kWarps + 2) {
         fence_after_sync();
         tmem_free(tmem, 512);
+        if (lane == 0) report_stall(broken, p.stalled);
     }
 }
 

@@ -534,6 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kSoftmaxWarps + 2) {
         fence_after_sync();
         tmem_free(tmem, 512);
+        if (lane == 0) report_stall(broken, p.stalled);
     }
 }
 

@@ -20,6 +20,11 @@ struct DeviceInfo {
 };
 DeviceInfo device_info(int device);
 
+// The word of policy_stall_word, allocated at the first call; null where that fails.
+int32_t* stall_word();
+// POLICY_ERR_STALLED, once, after a kernel has set it.
+int check_stall();
+
 // Makes `device` the calling thread's current device for the scope and puts the caller's
 // current device back when the scope ends.
 class DeviceScope {

@@ -48,17 +48,17 @@ __device__ __forceinline__ uint64_t nanoseconds()
 }
 
 // A wait lasts as long as a few tiles' work, microseconds.  One of two seconds can only come from a
-// defect: it raises the block's flag, on which every role leaves its loop.
+// defect: it raises the block's flag, on which every role leaves its loop, and the host's word at the end.
 constexpr uint64_t kWaitLimit = 2'000'000'000ull;
 
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* broken)
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* broken, uint64_t limit = kWaitLimit)
 {
     if (bar_try(bar, parity)) return true;
     const uint64_t start = nanoseconds();
     for (;;) {
         if (bar_try(bar, parity)) return true;
         if (*broken) return false;
-        if (nanoseconds() - start > kWaitLimit) {
+        if (nanoseconds() - start > limit) {
             *broken = 1;
             return false;
         }
@@ -69,6 +69,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* broken)
 {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, broken));
+}
+
+// By one thread of the block after its last barrier: tells the host that a wait ran out.
+__device__ __forceinline__ void report_stall(const volatile int* broken, int32_t* word)
+{
+    if (!*broken) return;
+    *static_cast<volatile int32_t*>(word) = 1;
+    __threadfence_system();
 }
 
 // Makes what the calling thread wrote to shared memory visible to the tensor core.
