@@ -29,7 +29,7 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Whether the phase is over; the hardware may hold the thread for up to some microseconds until it is.
+// Whether the phase is over; the hardware holds the thread for some microseconds until it is.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
 {
     uint32_t done;
@@ -40,29 +40,23 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
         : "=r"(done) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ uint64_t nanoseconds()
-{
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
-    return t;
-}
 
-// A wait lasts as long as a few tiles' work, microseconds.  One of two seconds can only come from a
-// defect: it raises the block's flag, on which every role leaves its loop, and the host's word at the end.
-constexpr uint64_t kWaitLimit = 2'000'000'000ull;
+// A wait lasts as long as a few tiles' work, microseconds.  One of two seconds' polls can only come from a defect: it
+// raises the block's flag, on which every role leaves its loop, and the host's word at the end.  It counts polls, not the
+// clock, which goes on while a context is paused (by a debugger, or for another process).
+constexpr uint32_t kPollNs = 32'768;  // how long a poll that fails is held (measured)
+constexpr uint32_t kWaitPolls = 2'000'000'000 / kPollNs;
 
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* broken, uint64_t limit = kWaitLimit)
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* broken, uint32_t polls = kWaitPolls)
 {
     if (bar_try(bar, parity)) return true;
-    const uint64_t start = nanoseconds();
-    for (;;) {
+#pragma unroll 1
+    for (uint32_t n = 0; n < polls; ++n) {
         if (bar_try(bar, parity)) return true;
         if (*broken) return false;
-        if (nanoseconds() - start > limit) {
-            *broken = 1;
-            return false;
-        }
     }
+    *broken = 1;
+    return false;
 }
 
 // The same for a whole warp, with one answer.

@@ -44,3 +44,17 @@ def test_a_wait_that_runs_out_is_an_error_of_the_next_call():
     with pytest.raises(RuntimeError, match="ran out of time"):
         torch.autograd.grad(out, q, out)
     torch.autograd.grad(policy.cross_attention(q, k, k), q, out)
+
+
+def test_polls_last_as_long_as_the_limit_takes_them_to():
+    """The limit counts polls, so that the time for which a context is paused is none of it."""
+    torch.cuda.init()
+    address = _native.policy_lib().policy_stall_word()
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    assert not wait(-1, 1_000_000, address)
+    begin.record()
+    assert not wait(-1, 200_000_000, address)
+    end.record()
+    end.synchronize()
+    ctypes.cast(address, ctypes.POINTER(ctypes.c_int32))[0] = 0
+    assert 100 < begin.elapsed_time(end) < 400
