@@ -307,6 +307,13 @@ def policy_lib() -> ctypes.CDLL:
     return _policy
 
 
+def policy_torch_fits(path: Path = POLICY_TORCH_PATH) -> bool:
+    """Whether the module at ``path`` was built for the installed torch (no other release has its ABI)."""
+    import torch
+
+    return f"navi_policy_torch for torch {torch.__version__}\0".encode() in path.read_bytes()
+
+
 def policy_torch() -> ModuleType:
     """The policy operators on torch tensors; raises RuntimeError when the module is not built or cannot load."""
     global _policy_torch
@@ -319,6 +326,11 @@ def policy_torch() -> ModuleType:
                     )
                 import torch  # noqa: F401  (its libraries resolve the module's symbols)
 
+                if not policy_torch_fits():
+                    raise RuntimeError(
+                        f"navi_b200 policy operators at {POLICY_TORCH_PATH} were not built for torch {torch.__version__}; "
+                        "run `python -m navi_b200.build`"
+                    )
                 name = POLICY_TORCH_PATH.stem
                 spec = importlib.util.spec_from_file_location(name, POLICY_TORCH_PATH)
                 try:

@@ -14,7 +14,7 @@
 - navi_policy_torch.so : those operators on torch tensors, with their autograd nodes (g++, torch's headers)
 - libnavi_probe.so : the L2 read-bandwidth probe of the benchmark's roofline
 
-All are rebuilt only when a source is newer than the library.
+All are rebuilt only when a source is newer than the library, and navi_policy_torch.so when torch is another.
 """
 
 from __future__ import annotations
@@ -25,6 +25,8 @@ import subprocess
 import sys
 import sysconfig
 from pathlib import Path
+
+from . import _native
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
@@ -147,7 +149,7 @@ def build_policy_torch(force: bool = False) -> Path:
     """navi_policy_torch.so: the Python module that puts libnavi_policy.so to work on torch tensors."""
     out = LIB / "navi_policy_torch.so"
     src = CSRC / "policy_torch.cpp"
-    if force or _stale(out, [src, INCLUDE / "policy.h"]):
+    if force or _stale(out, [src, INCLUDE / "policy.h"]) or not _native.policy_torch_fits(out):
         import torch
         from torch.utils import cpp_extension
 
@@ -157,7 +159,7 @@ def build_policy_torch(force: bool = False) -> Path:
         tmp = out.with_suffix(".so.tmp")
         _run([
             host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DNAVI_TORCH_VERSION="{torch.__version__}"',
             *(f"-isystem{d}" for d in cpp_extension.include_paths()), f"-I{sysconfig.get_paths()['include']}",
             f"-I{cuda / 'include'}", f"-I{INCLUDE}", str(src), "-o", str(tmp),
             f"-L{LIB}", "-lnavi_policy", "-Wl,-rpath,$ORIGIN",

@@ -394,6 +394,9 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const s
 
 }  // namespace
 
+// What the module was built for; the loader and the build look for it in the file.
+extern "C" __attribute__((used)) const char navi_policy_torch_built_for[] = "navi_policy_torch for torch " NAVI_TORCH_VERSION;
+
 PYBIND11_MODULE(navi_policy_torch, m)
 {
     using release = py::call_guard<py::gil_scoped_release>;
