@@ -114,7 +114,6 @@ struct Mma<bf16> {
         return *reinterpret_cast<const uint32_t*>(&v);
     }
     static __device__ __forceinline__ void store2(bf16* p, float a, float b) { *reinterpret_cast<uint32_t*>(p) = pack(a, b); }
-    static __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
 };
 
 // The k order inside a step is free as long as A and B share it: slot i < 4 holds k = 2i and
@@ -184,7 +183,6 @@ struct Mma<float> {
     {
         *reinterpret_cast<float2*>(p) = make_float2(a, b);
     }
-    static __device__ __forceinline__ float to_float(float v) { return v; }
 };
 
 __device__ __forceinline__ float quad_max(float v)
