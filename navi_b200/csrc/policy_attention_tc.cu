@@ -442,8 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float2 e = fma2(make_float2(now[2 * j], now[2 * j + 1]), c2, b2);
                         e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                         w[j] = Mma<bf16>::pack(e.x, e.y);
-                        // the sum is of the weights that multiply v
-                        sum = add2(sum, make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+                        add_bf16(sum, w[j]);  // the sum is of the weights that multiply v
                     }
                     tmem_store16(tp + q * 16, w);
                     if (q & 1) {

@@ -220,12 +220,11 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
+// sum += the two bf16 of w, in f32: without unpacking them first, which cost the forward pass 2 to 3 %
+__device__ __forceinline__ void add_bf16(float2& sum, uint32_t w)
 {
-    float2 r;
-    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
+    asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\nadd.rn.f32.bf16 %0, lo, %0;\nadd.rn.f32.bf16 %1, hi, %1;\n}\n"
+        : "+f"(sum.x), "+f"(sum.y) : "r"(w));
 }
 __device__ __forceinline__ float2 same(float v) { return make_float2(v, v); }
 
