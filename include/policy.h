@@ -61,8 +61,8 @@ POLICY_API const char* policy_last_error(void);
  * 16-byte aligned rows (base address, and strides times the element size).  out, dq, dk
  * and dv are contiguous; For the backward pass the
  * forward writes, where the pointers are not null, stats [batch][lq][heads][2] f32 (the exponent that its
- * weights are relative to, in base 2, and the reciprocal of their sum, 0 for a query that gives 0: a single
- * logarithm of the sum would carry its own rounding into every weight), and with POLICY_BF16 out_rest, bf16 in
+ * weights are relative to, in base 2, and the reciprocal of the sum of the weights as they multiply v, 0 for a
+ * query that gives 0: a single logarithm of the sum would carry its own rounding into every weight), and with POLICY_BF16 out_rest, bf16 in
  * the layout of out: what the rounding of out left off (dout . out in 8 bits would be the largest error of dq
  * and dk where a query sees few keys; null in the backward: taken as 0). */
 typedef struct policy_attention {

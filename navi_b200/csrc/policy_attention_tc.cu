@@ -16,8 +16,8 @@
 //
 // O is kept relative to a reference maximum that follows the running one only when it falls 8 (a factor of
 // 256) behind: the sums lose nothing in f32, P stays below 2^8 in bf16, and almost no tile pays for rescaling O.
-// Measured: 16 x 8 heads of 12,288 rows x 768 keys x 128 in 757 us, 817 TFLOP/s; 12,288 keys: 1,129 TFLOP/s; 4,096 x 768
-// x 64: 447 TFLOP/s.  What is left of the tensor cores' rate goes to the softmax between a tile's two products.
+// Measured: 16 x 8 heads of 12,288 rows x 768 keys x 128 in 753 us, 821 TFLOP/s; 4 x 8 heads of 12,288 rows and keys: 1,085
+// TFLOP/s; 8 x 8 heads of 4,096 x 768 x 64: 433 TFLOP/s.  What is left of the tensor cores' rate goes to the softmax between a tile's two products.
 // The special function unit gives 16 exponentials a clock and SM: as many clocks for a tile as its products
 // take at dim 128, twice as many at 64.  Replacing a part of them by polynomials on the multiply-add pipes was
 // slower at every share (2 of 8: 2 % at 12,288 x 768 x 128; 4 of 8: 14 %): the issue slots are the scarcer.

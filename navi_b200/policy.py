@@ -9,7 +9,7 @@
 The tensors are float32 or bfloat16 on a B200.  Every call is asynchronous on the caller's
 current CUDA stream and never synchronises the host; its outputs and scratch come from torch's
 allocator on that stream.  There is no CPU path: a missing native library or a non-CUDA tensor raises
-RuntimeError, and so does an argument of the wrong shape or type.  Derivatives are those of reverse mode:
+RuntimeError, and so does a tensor of the wrong shape or dtype (what is no tensor: TypeError).  Derivatives are those of reverse mode:
 a tensor that carries a forward-mode tangent raises RuntimeError, and so does a call inside ``torch.jit.trace``.
 """
 
@@ -55,7 +55,8 @@ def cross_attention(
 
     Returns [batch, lq, heads, dim], contiguous; differentiable once in q, k and v.  Scores,
     softmax and sums are held in 32 bits; with bfloat16 the softmax weights enter the product with
-    v (and with their gradients that with q and k) in bfloat16, and the outputs are rounded once.
+    v (and with their gradients that with q and k) in bfloat16, are divided by their own sum, and the outputs
+    are rounded once.
     Tensors whose rows are not dense and 16-byte aligned are copied first.
     """
     return _call("cross_attention", q, k, v, key_mask, key_lengths, scale)
