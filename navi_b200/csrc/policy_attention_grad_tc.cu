@@ -6,9 +6,10 @@
 // For every Y:  S = X_a Y_a^T,  T = X_b Y_b^T  (128 x 64, f32 in tensor memory), then a thread to a row of X
 //   p = 2^(c s - x_i) y_i,   ds = p (t - D_i)
 // written as bf16 over S and T (0.0024 of the gradients' norm off with it, 0.0017 of that from their own rounding), and
-// the products  dv += P dO, dk += dS Q  (or dq += dS K) with the left operand from tensor memory.  dv, dk and dq stay in tensor memory for the whole item.  A block has two sets (one where
-// tensor memory has no room for two: dk and dv at dim 128), each with 4 warps and its own product-issuing thread,
-// so that one set's products run during the other's arithmetic.  Blocks are persistent, one per SM.
+// the products  dv += P dO, dk += dS Q  (or dq += dS K) with the left operand from tensor memory.  dv, dk and dq stay in
+// tensor memory for the whole item.  A block has two sets (one where tensor memory has no room for two: dk and dv at dim
+// 128), each with 4 warps and its own product-issuing thread, so that one set's products run during the other's
+// arithmetic.  Blocks are persistent, one per SM.
 //
 // All tiles come by TMA, a row tile as 64 / group tokens x group heads.  One warp follows the copies of Y: for dq
 // it zeroes K's invisible rows (0 x NaN would be NaN) and says which keys are visible, for dk and dv it brings the
